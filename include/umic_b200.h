@@ -44,10 +44,13 @@ extern "C" {
 /* Device-side error bits, read with umic_device_errors(). */
 #define UMIC_DEVERR_KV_OVERFLOW 1u   /* device-position KV append out of range */
 #define UMIC_DEVERR_WAIT_TIMEOUT 2u  /* a bounded mbarrier wait ran out */
+#define UMIC_DEVERR_PAGES 4u         /* a request of umic_paged_plan was not served */
+#define UMIC_DEVERR_BAD_PAGE 8u      /* a page, slot or length outside the page pool */
 
 /* dtype codes for optional fp32 side inputs */
 #define UMIC_DTYPE_BF16 0
 #define UMIC_DTYPE_FP32 1
+#define UMIC_DTYPE_E4M3 2 /* 8-bit cache pages only */
 
 /* GEMV flags */
 #define UMIC_GEMV_WEIGHTS_READY 1u /* weights not written by the preceding stream op */
@@ -196,6 +199,102 @@ UMIC_API int umic_qk_norm_rope_kv(
     void* k_buf, void* v_buf, int64_t buf_sb, int64_t buf_sh, int64_t buf_ss, int64_t capacity,
     int64_t pos, const int64_t* dpos, int64_t batch, int64_t seq, int32_t head_dim,
     void* stream);
+
+/* ---- paged KV cache -------------------------------------------------------- */
+/* The three calls below serve requests of different lengths from one pool of pages.
+ * k_pages / v_pages are [num_pages, kv_heads, page_size, head_dim] through (pg_sp,
+ * pg_sh, pg_ss) element strides, K and V with the same strides, bf16 or e4m3 (with one
+ * fp32 scale per KV head: value = stored * scale; NULL = 1). A request's tokens
+ * [i * page_size, (i + 1) * page_size) live in page block_table[request, i]; the slot
+ * of a token is page * page_size + its place in the page. No reference counterpart:
+ * the reference keeps one dense buffer per layer whose rows share a length
+ * (src/umic/cache.py:25-160). */
+
+/* One serving step's bookkeeping on the device, from request lengths: grows or shrinks
+ * every request's row of the block table and says where the step's new tokens go.
+ * kv_lens [requests] holds the cached lengths, new_tokens [requests] the change: n > 0
+ * appends n tokens, n < 0 drops the last -n (-kv_lens[i] ends the request). The free
+ * pages are a ring: free_ring[i % num_pages] for free_span[0] <= i < free_span[1].
+ * With pages(x) = ceil(x / page_size), in request order:
+ *   valid   kv_lens and kv_lens + new_tokens >= 0, pages of both <= max_pages
+ *   served  valid, and the pages needed by the valid requests up to this one fit the
+ *           free pages (or it needs none), and the tokens appended by them fit
+ *           `capacity` (or it appends none)
+ * A served request takes its pages from the front of the ring, gives the pages that
+ * hold no more tokens back at its end, and its length changes; a request that is not
+ * served keeps all it had and sets UMIC_DEVERR_PAGES. Outputs: out_lens [requests];
+ * out_span [2]; cu_tokens [requests + 1], where each valid request's appended tokens
+ * begin among the step's tokens (held at 2^31 - 1 past it); slots and positions
+ * [capacity], the slot and the position in its request of each of the step's tokens, -1
+ * for the tokens of requests not served and behind the last (and where a page taken
+ * from the ring or the table is outside the pool, with UMIC_DEVERR_BAD_PAGE). block_table (rows
+ * table_stride apart) and free_ring change in place; entries behind a row's length keep
+ * what they held. out_lens may be kv_lens and out_span may be free_span; the other
+ * arrays may not overlap. Calls on one pool must be ordered on one stream. requests at
+ * most 8192; num_pages * page_size, max_pages * page_size and capacity below 2^31. */
+UMIC_API int umic_paged_plan(const int32_t* kv_lens, const int32_t* new_tokens,
+                             int64_t requests, int32_t* block_table, int64_t table_stride,
+                             int64_t max_pages, int32_t* free_ring, int64_t num_pages,
+                             const int64_t* free_span, int64_t page_size, int32_t* out_lens,
+                             int64_t* out_span, int32_t* cu_tokens, int32_t* slots,
+                             int32_t* positions, int64_t capacity, void* stream);
+
+/* Attention input of ragged tokens in one pass: per-head RMSNorm (NULL weight = none),
+ * rotate-half RoPE with several position axes, and the write of K and V into pages.
+ * q [tokens, hq, head_dim] through (q_st, q_sh), k and v with hk heads; q_out (which
+ * may be q itself) gets the rotated q. With k_pages, K and V of token t are written at
+ * slots[t] (-1: not written; other slots outside the pool set UMIC_DEVERR_BAD_PAGE and
+ * are not written; two tokens must not share a slot), rounded once to cache_dtype (e4m3
+ * saturates at +-448); without, the rotated k goes to k_out (which may be k) and v is
+ * not touched. The angle of pair i, which holds elements i and i + rotary_dim / 2, is
+ * positions[axis(i), t] * inv_freq[i], computed in 64 bits: axis(i) = the section of
+ * (s0, s1, s2) that i falls in, or with interleaved != 0 (t h w t h w ... t t) axis
+ * i % axes while i < axes * s_axis, else axis 0. Sections sum to rotary_dim / 2; cos
+ * and sin are multiplied by scaling; elements from rotary_dim on are passed through.
+ * positions [axes, tokens] through (p_sa, p_st; 0 broadcasts), int32 or int64
+ * (pos_bytes 4 or 8). rotary_dim 0: no rotation (positions, inv_freq unused). hq 0:
+ * no q. head_dim a multiple of 16 up to 256, rotary_dim a multiple of 16 up to it.
+ * Replaces, as one kernel, q_norm / k_norm (integrate.py:134-141), the three-axis
+ * cos/sin tables of transformers' rotary module, apply_rotary_pos_emb (rope.py:86-107)
+ * or apply_rotary_vision_triton (rope.py:78-84), and the cache write
+ * (cache.py:59-60). */
+UMIC_API int umic_qk_norm_mrope_kv(
+    const void* q, int64_t q_st, int64_t q_sh, int32_t hq, const void* k, int64_t k_st,
+    int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, int32_t hk, void* q_out,
+    int64_t qo_st, int64_t qo_sh, void* k_out, int64_t ko_st, int64_t ko_sh,
+    const void* q_weight, const void* k_weight, int w_dtype, float q_eps, float k_eps,
+    const void* positions, int pos_bytes, int64_t p_sa, int64_t p_st, const float* inv_freq,
+    int32_t rotary_dim, int32_t axes, int32_t s0, int32_t s1, int32_t s2, int interleaved,
+    float scaling, void* k_pages, void* v_pages, int64_t pg_sp, int64_t pg_sh, int64_t pg_ss,
+    int64_t num_pages, int64_t page_size, int cache_dtype, const float* k_scale,
+    const float* v_scale, const int32_t* slots, int64_t tokens, int32_t head_dim,
+    void* stream);
+
+/* Attention of one new token per request over its pages, grouped-query heads:
+ * out[b, h] = softmax(scale * q[b, h] . k_j over j < kv_lens[b]) . v_j. q and out
+ * [batch, hq, head_dim] through (sb, sh); lse [batch, hq] fp32 (natural log of the sum
+ * of exponentials; NULL = not wanted). A request without tokens comes out as zeros,
+ * lse -inf. A table entry outside the pool is left out of its request's sums, a length
+ * past max_pages * page_size is cut there; both set UMIC_DEVERR_BAD_PAGE. What lies
+ * behind a request's length in its last page is never used. head_dim 64, 80, 96, 128 or
+ * 256, hq a multiple of hkv, page_size a multiple of 16, 16-byte aligned bases and
+ * strides. The lengths are read on the device: one captured graph serves every length.
+ * workspace: umic_paged_attention_workspace_bytes() bytes, 16-byte aligned, contents
+ * irrelevant before and after; calls that may overlap need one each.
+ * Replaces the SDPA call of the decode step (graph.py:76-99), for rows of different
+ * lengths. */
+UMIC_API int umic_paged_attention(
+    const void* q, int64_t q_sb, int64_t q_sh, const void* k_pages, const void* v_pages,
+    int64_t pg_sp, int64_t pg_sh, int64_t pg_ss, int64_t num_pages, int64_t page_size,
+    int cache_dtype, const float* k_scale, const float* v_scale, const int32_t* block_table,
+    int64_t table_stride, int64_t max_pages, const int32_t* kv_lens, void* out, int64_t o_sb,
+    int64_t o_sh, float* lse, int64_t batch, int32_t hq, int32_t hkv, int32_t head_dim,
+    float scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Bytes of workspace umic_paged_attention needs for these heads on the current device,
+ * whatever the batch and lengths. */
+UMIC_API size_t umic_paged_attention_workspace_bytes(int32_t hq, int32_t hkv,
+                                                     int32_t head_dim);
 
 /* ---- attention over a cached prefix -------------------------------------- */
 

@@ -69,6 +69,19 @@ _SIGNATURES: dict[str, list] = {
                             _c_f32, _c_p],
     "umic_mask_pack_bits": [_c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_p,
                             _c_i64, _c_i64, _c_i64, _c_p],
+    "umic_paged_plan": [_c_p, _c_p, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_i64,
+                        _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_p],
+    "umic_qk_norm_mrope_kv": [_c_p, _c_i64, _c_i64, _c_i32, _c_p, _c_i64, _c_i64, _c_p, _c_i64,
+                              _c_i64, _c_i32, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p,
+                              _c_p, _c_int, _c_f32, _c_f32, _c_p, _c_int, _c_i64, _c_i64, _c_p,
+                              _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_int, _c_f32, _c_p, _c_p,
+                              _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_int, _c_p, _c_p, _c_p,
+                              _c_i64, _c_i32, _c_p],
+    "umic_paged_attention": [_c_p, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64,
+                             _c_i64, _c_int, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p,
+                             _c_i64, _c_i64, _c_p, _c_i64, _c_i32, _c_i32, _c_i32, _c_f32, _c_p,
+                             _c_size, _c_p],
+    "umic_paged_attention_workspace_bytes": [_c_i32, _c_i32, _c_i32],
     "umic_gemm": [_c_p, _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_i64, _c_p, _c_i64, _c_i64, _c_i64,
                   _c_i64, _c_int, _c_p],
     "umic_gemm_ws": [_c_p, _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_i64, _c_p, _c_i64, _c_i64,
@@ -78,7 +91,8 @@ _SIGNATURES: dict[str, list] = {
                                 _c_i64, _c_i64, _c_p],
 }
 _RESTYPES = {"umic_last_error_message": ctypes.c_char_p, "umic_gemv_workspace_bytes": _c_size,
-             "umic_gemm_workspace_bytes": _c_size}
+             "umic_gemm_workspace_bytes": _c_size,
+             "umic_paged_attention_workspace_bytes": _c_size}
 
 ERR_NAMES = {1: "INVALID_ARG", 2: "UNSUPPORTED", 3: "ALIGNMENT", 4: "LAUNCH", 5: "OVERFLOW",
              6: "DEVICE"}
@@ -88,10 +102,13 @@ ERR_OVERFLOW = 5
 
 DTYPE_BF16 = 0
 DTYPE_FP32 = 1
+DTYPE_E4M3 = 2
 EPI_NONE, EPI_GELU_ERF, EPI_GELU_TANH = 0, 1, 2
 GEMV_WEIGHTS_READY = 1
 DEVERR_KV_OVERFLOW = 1
 DEVERR_WAIT_TIMEOUT = 2
+DEVERR_PAGES = 4
+DEVERR_BAD_PAGE = 8
 
 _lib = None
 _lock = threading.Lock()
