@@ -2,96 +2,771 @@
 //
 //   out[b, h] = sum_j softmax_j(scale q[b, h] . k_j) v_j,  j < kv_lens[b]
 //
-// One pass over K and V with a running maximum m and sum l: at a new score s,
-// m' = max(m, s), and the sum and the output accumulator are multiplied by
-// exp(m - m') before exp(s - m') and exp(s - m') v are added. A warp owns one query head.
+// Every K and V byte is used once, for the G query heads of its KV head: 2 G flops a byte
+// (bf16) against the hundreds that the tensor cores could do, so HBM bounds the kernel and
+// all that matters is to keep its loads in flight.
+//
+// Work. A segment is one request's one KV head (up to 8 * NT query heads; wider groups are
+// cut into several segments), a tile 16 of its tokens. All tiles of all segments form one
+// line, and every warp takes an equal run of it, whatever the lengths: no warp idles
+// because its request is short. A warp needs no other: it copies its tiles into its own
+// ring with 16-byte asynchronous loads, kStages ahead across segment borders, and waits for
+// its own copies only. Per tile:
+//   S^T = K Q^T    mma.sync m16n8k16, tokens as rows: the 8 columns are query heads, so a
+//                  group of up to 8 heads costs one instruction per 16 dims (tcgen05 wants
+//                  64 or 128 rows per operand and a block-wide hand-over of each tile;
+//                  here the tensor pipe is busy a few per cent of the time either way)
+//   m, l, P        running maximum and sum of each head, fp32, base 2
+//   O^T += V^T P   V through transposing ldmatrix, P transposed in registers
+// P is fp32 split into a bf16 value and its bf16 remainder (two products, weights held to
+// 2^-17): the tensor pipe has the time. e4m3 pages are widened to fp16 in registers, which
+// holds them exactly; q is scaled by a power of two to stay inside fp16 and P by 2^14 so
+// that small weights stay normal, rounded to 2^-12.
+//
+// Join. A warp whose run covers a whole segment writes its rows. Otherwise it has partial
+// (m, l, O): neighbours of one CTA that share a segment join through shared memory, and
+// what still crosses CTAs goes to the workspace, where a second kernel joins the partials
+// of each split segment in line order. Sums are taken in a fixed order: results repeat bit
+// for bit.
 #include <cuda_fp8.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "common.cuh"
+#include "mma_frag.cuh"
 
 namespace umic {
 namespace {
 
+constexpr int kTile = 16;             // tokens per tile
+constexpr float kF16Shift = 14.f;     // e4m3 path: weights are held as 2^14 p
+constexpr int kSmemBudget = 216 * 1024;
+constexpr int64_t kMaxWorkers = 2048;  // warps of the main kernel, bounds the workspace
+
 struct PagedArgs {
   const __nv_bfloat16* q;
-  const void *k_pages, *v_pages;
+  const char *k_pages, *v_pages;
   const float *k_scale, *v_scale;
   const int32_t *table, *lens;
   __nv_bfloat16* out;
   float* lse;
   uint32_t* err;
-  int64_t q_sb, q_sh, pg_sp, pg_sh, pg_ss, table_stride, max_len, num_pages, o_sb, o_sh;
-  int32_t page_size, hq, hkv, batch;
-  float scale;
+  float* ws;
+  int64_t q_sb, q_sh, pg_sp, pg_sh, pg_ss;  // pg_* in bytes
+  int64_t table_stride, max_len, num_pages, o_sb, o_sh;
+  int32_t page_size, hq, hkv, batch, group, chunks;  // chunks: segments per KV head
+  float scale_log2;
 };
 
-__device__ __forceinline__ float load_elem(const void* p, int64_t at, bool e4m3) {
-  if (!e4m3) return bf(static_cast<const __nv_bfloat16*>(p)[at]);
-  const __half_raw h =
-      __nv_cvt_fp8_to_halfraw(static_cast<const __nv_fp8_storage_t*>(p)[at], __NV_E4M3);
-  return __half2float(__half(h));
+// Shapes of one instantiation.
+template <int D, bool kE4m3, int NT>
+struct Shape {
+  static constexpr int kRow = D * (kE4m3 ? 1 : 2);                   // bytes of a token's row
+  static constexpr int kPitch = kRow + ((kRow / 16) % 2 ? 0 : 16);  // odd count of 16 B: no
+                                                                    // bank conflicts
+  static constexpr int kTileBytes = 2 * kTile * kPitch;             // K, then V
+  static constexpr int kWarps = D == 256 && !kE4m3 ? 4 : 8;
+  static constexpr int kFit = kSmemBudget / (kWarps * kTileBytes);
+  static constexpr int kStages = kFit < 6 ? kFit : 6;
+  static constexpr int kBlocks = D / 16;                            // 16-dim blocks
+  static constexpr int kOut = NT * kBlocks * 128;                   // floats of one partial O
+  static constexpr int kSlot = kOut + NT * 16;                      // + m and l of 8 * NT heads
+  static constexpr size_t kSmem = static_cast<size_t>(kWarps) * kStages * kTileBytes;
+  static_assert(kStages >= 2, "one tile in use, one in flight");
+  static_assert(kStages * kTileBytes >= kSlot * 4, "a partial result fits its warp's ring");
+};
+
+// A split segment, left by the warp that holds its first tile for the joining kernel.
+struct Split {
+  int32_t b;     // request, or -1: none begins here
+  int32_t hc;    // segment of the request
+  int32_t last;  // worker that holds its last tile
+  int32_t head;  // 1: that worker's run goes on behind the segment
+};
+
+__host__ __device__ constexpr int64_t slot_of(int64_t worker, int head) { return worker * 2 + head; }
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(there ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm2(uint32_t& r0, uint32_t& r1, uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0,%1}, [%2];"
+               : "=r"(r0), "=r"(r1)
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm2t(uint32_t& r0, uint32_t& r1, uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];"
+               : "=r"(r0), "=r"(r1)
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                        uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// two e4m3 values (low byte first) as fp16, exactly
+__device__ __forceinline__ uint32_t widen(uint32_t two) {
+  const __half2_raw h =
+      __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two & 0xffffu), __NV_E4M3);
+  return static_cast<uint32_t>(h.x) | static_cast<uint32_t>(h.y) << 16;
 }
 
-template <int D, bool kE4m3>
-__global__ void __launch_bounds__(32) paged_attn_kernel(PagedArgs a) {
+__device__ __forceinline__ int64_t clamped_len(const PagedArgs& a, int b) {
+  const int64_t n = a.lens[b];
+  return n < 0 ? 0 : n > a.max_len ? a.max_len : n;
+}
+
+// One warp's view of a segment's rows: where the outputs of its heads go.
+template <int D, bool kE4m3, int NT>
+struct Rows {
+  __device__ static int head0(const PagedArgs& a, int hc) {  // first query head of a segment
+    return hc / a.chunks * a.group + hc % a.chunks * (8 * NT);
+  }
+  __device__ static int heads(const PagedArgs& a, int hc) {
+    return min(8 * NT, a.group - hc % a.chunks * (8 * NT));
+  }
+  // Output block md of accumulator fragments: rows are dims, columns 2c and 2c + 1 heads;
+  // inv0 / inv1 normalise the two columns.
+  __device__ static void store(const PagedArgs& a, int b, int hc, int nt, int md,
+                               const float4& o, float inv0, float inv1, int lane) {
+    const int g = lane >> 2, c = lane & 3, n = heads(a, hc);
+    __nv_bfloat16* base = a.out + b * a.o_sb + static_cast<int64_t>(head0(a, hc)) * a.o_sh;
+    if constexpr (kE4m3) {  // rows g and g + 8 are dims 2g and 2g + 1
+      const int h = nt * 8 + 2 * c;
+      if (h < n)
+        *reinterpret_cast<uint32_t*>(base + h * a.o_sh + md * 16 + 2 * g) =
+            pack_bf16(o.x * inv0, o.z * inv0);
+      if (h + 1 < n)
+        *reinterpret_cast<uint32_t*>(base + (h + 1) * a.o_sh + md * 16 + 2 * g) =
+            pack_bf16(o.y * inv1, o.w * inv1);
+    } else {
+      const uint32_t lo = transpose8x8(pack_bf16(o.x * inv0, o.y * inv1));
+      const uint32_t hi = transpose8x8(pack_bf16(o.z * inv0, o.w * inv1));
+      const int h = nt * 8 + g;
+      if (h < n) {
+        *reinterpret_cast<uint32_t*>(base + h * a.o_sh + md * 16 + 2 * c) = lo;
+        *reinterpret_cast<uint32_t*>(base + h * a.o_sh + md * 16 + 8 + 2 * c) = hi;
+      }
+    }
+  }
+  __device__ static float inverse(const PagedArgs& a, int hc, float l) {
+    const float unit = kE4m3 && a.v_scale ? a.v_scale[hc / a.chunks] : 1.f;
+    return l == 0.f ? 0.f : unit / l;
+  }
+  __device__ static void store_lse(const PagedArgs& a, int b, int hc, int nt, float m0, float l0,
+                                   float m1, float l1, int lane) {
+    if (!a.lse || lane >= 4) return;
+    const int h = nt * 8 + 2 * lane, n = heads(a, hc);
+    float* base = a.lse + static_cast<int64_t>(b) * a.hq + head0(a, hc);
+    constexpr float kLn2 = 0.693147180559945309f, shift = kE4m3 ? kF16Shift : 0.f;
+    if (h < n) base[h] = l0 == 0.f ? -INFINITY : (m0 - shift) * kLn2 + logf(l0);
+    if (h + 1 < n) base[h + 1] = l1 == 0.f ? -INFINITY : (m1 - shift) * kLn2 + logf(l1);
+  }
+};
+
+// weight of a partial result with maximum m among ones with maximum `top`
+__device__ __forceinline__ float weight_of(float m, float top) {
+  return m == -INFINITY ? 0.f : exp2_fast(m - top);
+}
+
+template <int D, bool kE4m3, int NT>
+__global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
+    paged_attn_kernel(PagedArgs a) {
+  using S = Shape<D, kE4m3, NT>;
+  using R = Rows<D, kE4m3, NT>;
+  constexpr int kWarps = S::kWarps, kStages = S::kStages, kBlocks = S::kBlocks;
+  constexpr int kThreads = kWarps * 32;
+  extern __shared__ __align__(16) char ring_mem[];
+  __shared__ int4 s_info[kWarps][kStages];  // request, segment, valid rows, tiles left
+  __shared__ int4 s_begin[kWarps];          // request, segment, tile at a warp's start
+  __shared__ int64_t s_warp_sum[kWarps];
+  __shared__ int4 s_tail[kWarps];  // has a tail | 2 starts it | 4 ends it, request, segment
+  __shared__ Split s_split[kWarps];
+
   allow_dependent_launch();
   wait_prerequisite();
-  constexpr int kPer = (D + 31) / 32;
-  const int lane = threadIdx.x;
-  const int b = blockIdx.x / a.hq, h = blockIdx.x % a.hq, hk = h / (a.hq / a.hkv);
-  int64_t len = a.lens[b];
-  if (len > a.max_len || len < 0) {
-    if (lane == 0) atomicOr(a.err, UMIC_DEVERR_BAD_PAGE);
-    len = len < 0 ? 0 : a.max_len;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int hcs = a.hkv * a.chunks;  // segments per request
+
+  // ---- the line of tiles, and where each warp's run begins on it
+  const int per = (a.batch + kThreads - 1) / kThreads;
+  const int b0 = min(a.batch, static_cast<int>(threadIdx.x) * per), b1 = min(a.batch, b0 + per);
+  int64_t mine = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int64_t n = a.lens[b];
+    if (blockIdx.x == 0 && (n < 0 || n > a.max_len)) atomicOr(a.err, UMIC_DEVERR_BAD_PAGE);
+    mine += (clamped_len(a, b) + kTile - 1) / kTile;
   }
-  float q[kPer], o[kPer];
-  for (int i = 0; i < kPer; ++i) {
-    const int e = lane + 32 * i;
-    q[i] = e < D ? bf(a.q[b * a.q_sb + h * a.q_sh + e]) : 0.f;
-    o[i] = 0.f;
+  int64_t upto = mine;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += x;
   }
-  const float scale = a.scale * (a.k_scale ? a.k_scale[hk] : 1.f);
-  float m = -INFINITY, l = 0.f;
-  for (int64_t j = 0; j < len; ++j) {
-    const int64_t page = a.table[b * a.table_stride + j / a.page_size];
-    if (page < 0 || page >= a.num_pages) {
-      if (lane == 0) atomicOr(a.err, UMIC_DEVERR_BAD_PAGE);
-      continue;
+  if (lane == 31) s_warp_sum[warp] = upto;
+  __syncthreads();
+  int64_t total = 0;
+  upto -= mine;
+  for (int w = 0; w < kWarps; ++w) {
+    if (w == warp) upto += total;
+    total += s_warp_sum[w];
+  }
+  total *= hcs;
+  const int64_t workers = min(static_cast<int64_t>(gridDim.x) * kWarps, total);
+  const int64_t first_worker = static_cast<int64_t>(blockIdx.x) * kWarps;
+  for (int w = 0; w < kWarps && first_worker + w < workers; ++w) {
+    const int64_t at = (first_worker + w) * total / workers;
+    if (at < upto * hcs || at >= (upto + mine) * hcs) continue;
+    int64_t from = upto * hcs;
+    for (int b = b0; b < b1; ++b) {
+      const int64_t tiles = (clamped_len(a, b) + kTile - 1) / kTile;
+      if (at < from + tiles * hcs) {
+        s_begin[w] = make_int4(b, static_cast<int>((at - from) / tiles),
+                               static_cast<int>((at - from) % tiles), 0);
+        break;
+      }
+      from += tiles * hcs;
     }
-    const int64_t at = page * a.pg_sp + hk * a.pg_sh + j % a.page_size * a.pg_ss;
-    float s = 0.f;
-    for (int i = 0; i < kPer; ++i) {
-      const int e = lane + 32 * i;
-      if (e < D) s += q[i] * load_elem(a.k_pages, at + e, kE4m3);
-    }
-    for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    s *= scale;
-    const float top = fmaxf(m, s);
-    const float keep = m == -INFINITY ? 0.f : expf(m - top);
-    const float p = top == -INFINITY ? 0.f : expf(s - top);
-    m = top;
-    l = l * keep + p;
-    for (int i = 0; i < kPer; ++i) {
-      const int e = lane + 32 * i;
-      if (e < D) o[i] = o[i] * keep + p * load_elem(a.v_pages, at + e, kE4m3);
-    }
   }
-  const float inv = l == 0.f ? 0.f : (a.v_scale ? a.v_scale[hk] : 1.f) / l;
-  for (int i = 0; i < kPer; ++i) {
-    const int e = lane + 32 * i;
-    if (e < D) a.out[b * a.o_sb + h * a.o_sh + e] = __float2bfloat16_rn(o[i] * inv);
+  // requests without tokens: zeros
+  for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
+    if (clamped_len(a, b) > 0) continue;
+    for (int i = threadIdx.x; i < a.hq * (D / 8); i += kThreads)
+      st_vec(a.out + b * a.o_sb + i / (D / 8) * a.o_sh + i % (D / 8) * 8, make_uint4(0, 0, 0, 0));
+    if (a.lse)
+      for (int h = threadIdx.x; h < a.hq; h += kThreads)
+        a.lse[static_cast<int64_t>(b) * a.hq + h] = -INFINITY;
   }
-  if (a.lse && lane == 0)
-    a.lse[static_cast<int64_t>(b) * a.hq + h] = l == 0.f ? -INFINITY : m + logf(l);
+  __syncthreads();
+
+  const int64_t worker = first_worker + warp;
+  const int64_t begin = worker < workers ? worker * total / workers : 0;
+  const int64_t end = worker < workers ? (worker + 1) * total / workers : 0;
+  const int count = static_cast<int>(end - begin);
+  char* const ring = ring_mem + static_cast<size_t>(warp) * kStages * S::kTileBytes;
+  const uint32_t ring_addr = smem_addr(ring);
+
+  // ---- loader: the next tile to copy
+  int lb = 0, lhc = 0, lt = 0, ltiles = 0, lpi = 0, loff = 0;
+  int64_t llen = 0;
+  int32_t lpage = 0;
+  if (count > 0) {
+    const int4 st = s_begin[warp];
+    lb = st.x;
+    lhc = st.y;
+    lt = st.z;
+    llen = clamped_len(a, lb);
+    ltiles = static_cast<int>((llen + kTile - 1) / kTile);
+    lpi = lt * kTile / a.page_size;
+    loff = lt * kTile % a.page_size;
+    lpage = a.table[lb * a.table_stride + lpi];
+  }
+  int loaded = 0;
+  auto load = [&](int stage) {
+    if (loaded < count) {
+      ++loaded;
+      int rows = static_cast<int>(min(static_cast<int64_t>(kTile), llen - static_cast<int64_t>(lt) * kTile));
+      int64_t page = lpage;
+      if (page < 0 || page >= a.num_pages) {
+        if (lane == 0) atomicOr(a.err, UMIC_DEVERR_BAD_PAGE);
+        page = 0;
+        rows = 0;
+      }
+      if (lane == 0) s_info[warp][stage] = make_int4(lb, lhc, rows, ltiles - lt);
+      const int64_t base = page * a.pg_sp + lhc / a.chunks * a.pg_sh + loff * a.pg_ss;
+      const uint32_t dst = ring_addr + stage * S::kTileBytes;
+      constexpr int kCols = S::kRow / 16;  // 16-byte pieces of a row
+#pragma unroll
+      for (int i = 0; i < (kTile * kCols + 31) / 32; ++i) {
+        const int x = i * 32 + lane, row = x / kCols, col = x % kCols;
+        if ((kTile * kCols) % 32 != 0 && row >= kTile) break;
+        // rows behind the length are filled with zeros: a weight of 0 times what an
+        // unwritten page holds could be NaN
+        const bool there = row < rows;
+        const int64_t at = base + (there ? row * a.pg_ss + col * 16 : 0);
+        cp_async16(dst + row * S::kPitch + col * 16, a.k_pages + at, there);
+        cp_async16(dst + kTile * S::kPitch + row * S::kPitch + col * 16, a.v_pages + at, there);
+      }
+      if (loaded < count) {  // step on; the page is fetched now and used by the next call
+        if (++lt == ltiles) {
+          lt = lpi = loff = 0;
+          if (++lhc == hcs) {
+            lhc = 0;
+            do llen = clamped_len(a, ++lb);
+            while (llen == 0);
+            ltiles = static_cast<int>((llen + kTile - 1) / kTile);
+          }
+          lpage = a.table[lb * a.table_stride];
+        } else if ((loff += kTile) == a.page_size) {
+          loff = 0;
+          lpage = a.table[lb * a.table_stride + ++lpi];
+        }
+      }
+    }
+    cp_commit();
+  };
+
+  // ---- one segment's state
+  const int g = lane >> 2, c = lane & 3;
+  uint32_t qf[NT][kBlocks][2];
+  float o[NT][kBlocks][4];
+  float m[NT][2], l[NT][2], fac[NT][2];
+  int sb = 0, shc = 0;
+  bool open = false, from_start = false;
+  int64_t seg_end = 0;  // line position behind the segment
+
+  auto begin_segment = [&](int b, int hc) {
+    sb = b;
+    shc = hc;
+    const int n = R::heads(a, hc);
+    const __nv_bfloat16* q = a.q + b * a.q_sb + static_cast<int64_t>(R::head0(a, hc)) * a.q_sh;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int h = nt * 8 + g;
+      const __nv_bfloat16* row = q + h * a.q_sh;
+      if constexpr (!kE4m3) {
+#pragma unroll
+        for (int k = 0; k < kBlocks; ++k) {
+          qf[nt][k][0] = h < n ? *reinterpret_cast<const uint32_t*>(row + k * 16 + 2 * c) : 0u;
+          qf[nt][k][1] = h < n ? *reinterpret_cast<const uint32_t*>(row + k * 16 + 8 + 2 * c) : 0u;
+        }
+        fac[nt][0] = fac[nt][1] = a.scale_log2;
+      } else {
+        // a lane's four bytes of a K row are dims 4c .. 4c + 3 of a block: q to match,
+        // scaled by the power of two of its largest value
+        uint2 raw[kBlocks];
+        float top = 0.f;
+#pragma unroll
+        for (int k = 0; k < kBlocks; ++k) {
+          raw[k] = h < n ? *reinterpret_cast<const uint2*>(row + k * 16 + 4 * c) : make_uint2(0, 0);
+          top = fmaxf(top, fmaxf(fabsf(__uint_as_float(raw[k].x << 16)),
+                                 fabsf(__uint_as_float(raw[k].x & 0xffff0000u))));
+          top = fmaxf(top, fmaxf(fabsf(__uint_as_float(raw[k].y << 16)),
+                                 fabsf(__uint_as_float(raw[k].y & 0xffff0000u))));
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // 2^e <= top < 2^(e + 1); e kept where 2^-e is a normal number
+        const int e = top > 0.f && top < INFINITY
+                          ? max(-126, min(126, static_cast<int>(__float_as_uint(top) >> 23) - 127))
+                          : 0;
+        const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+        const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+#pragma unroll
+        for (int k = 0; k < kBlocks; ++k) {
+          qf[nt][k][0] = pack_f16(__uint_as_float(raw[k].x << 16) * down,
+                                  __uint_as_float(raw[k].x & 0xffff0000u) * down);
+          qf[nt][k][1] = pack_f16(__uint_as_float(raw[k].y << 16) * down,
+                                  __uint_as_float(raw[k].y & 0xffff0000u) * down);
+        }
+        const float f = a.scale_log2 * (a.k_scale ? a.k_scale[hc / a.chunks] : 1.f) * up;
+        fac[nt][0] = __shfl_sync(0xffffffffu, f, 8 * c);
+        fac[nt][1] = __shfl_sync(0xffffffffu, f, 8 * c + 4);
+      }
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+      for (int k = 0; k < kBlocks; ++k) o[nt][k][0] = o[nt][k][1] = o[nt][k][2] = o[nt][k][3] = 0.f;
+    }
+  };
+
+  auto tile = [&](int stage, int rows) {
+    const uint32_t kt = ring_addr + stage * S::kTileBytes, vt = kt + kTile * S::kPitch;
+    float s[NT][2][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[nt][0][j] = s[nt][1][j] = 0.f;
+    // two accumulators: half the chain of dependent products
+    if constexpr (!kE4m3) {
+      const uint32_t at = kt + ((lane & 7) + (lane & 8)) * S::kPitch + (lane >> 4) * 16;
+#pragma unroll
+      for (int k = 0; k < kBlocks; ++k) {
+        uint32_t r[4];
+        ldsm4(r, at + k * 32);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          mma16816(s[nt][k & 1], r[0], r[1], r[2], r[3], qf[nt][k][0], qf[nt][k][1]);
+      }
+    } else {
+      const uint32_t at = kt + ((lane & 7) + (lane & 8)) * S::kPitch;
+#pragma unroll
+      for (int k = 0; k < kBlocks; k += 2) {
+        uint32_t r[4];
+        if (k + 1 < kBlocks) ldsm4(r, at + k * 16 + (lane >> 4) * 16);
+        else ldsm2(r[0], r[1], at + k * 16);
+#pragma unroll
+        for (int u = 0; u < 2 && k + u < kBlocks; ++u) {
+          const uint32_t a0 = widen(r[2 * u]), a1 = widen(r[2 * u + 1]);
+          const uint32_t a2 = widen(r[2 * u] >> 16), a3 = widen(r[2 * u + 1] >> 16);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            mma_f16(s[nt][u], a0, a1, a2, a3, qf[nt][k + u][0], qf[nt][k + u][1]);
+        }
+      }
+    }
+    uint32_t ph[NT][2], pl[NT][2];
+    bool moved = false;
+    float keep[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = (s[nt][0][j] + s[nt][1][j]) * fac[nt][j & 1];
+      if (rows < kTile) {
+        if (g >= rows) x[0] = x[1] = -INFINITY;
+        if (g + 8 >= rows) x[2] = x[3] = -INFINITY;
+      }
+      float top[2] = {fmaxf(x[0], x[2]), fmaxf(x[1], x[3])};
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) {
+        top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], d));
+        top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], d));
+      }
+      float ref[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        top[j] = fmaxf(top[j], m[nt][j]);
+        ref[j] = top[j] == -INFINITY ? 0.f : top[j];
+        keep[nt][j] = exp2_fast(m[nt][j] - ref[j]);
+        moved |= keep[nt][j] != 1.f;
+        m[nt][j] = top[j];
+        if constexpr (kE4m3) ref[j] -= kF16Shift;
+      }
+      float p[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) p[j] = exp2_fast(x[j] - ref[j & 1]);
+      l[nt][0] = l[nt][0] * keep[nt][0] + (p[0] + p[2]);
+      l[nt][1] = l[nt][1] * keep[nt][1] + (p[1] + p[3]);
+      if constexpr (kE4m3) {
+        ph[nt][0] = transpose8x8(pack_f16(p[0], p[1]));
+        ph[nt][1] = transpose8x8(pack_f16(p[2], p[3]));
+      } else {
+        const uint32_t h0 = pack_bf16(p[0], p[1]), h1 = pack_bf16(p[2], p[3]);
+        ph[nt][0] = transpose8x8(h0);
+        ph[nt][1] = transpose8x8(h1);
+        pl[nt][0] = transpose8x8(pack_bf16(p[0] - __uint_as_float(h0 << 16),
+                                           p[1] - __uint_as_float(h0 & 0xffff0000u)));
+        pl[nt][1] = transpose8x8(pack_bf16(p[2] - __uint_as_float(h1 << 16),
+                                           p[3] - __uint_as_float(h1 & 0xffff0000u)));
+      }
+    }
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int k = 0; k < kBlocks; ++k)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[nt][k][j] *= keep[nt][j & 1];
+    }
+    if constexpr (!kE4m3) {
+      const uint32_t at = vt + ((lane & 7) + ((lane >> 4) << 3)) * S::kPitch + ((lane >> 3) & 1) * 16;
+#pragma unroll
+      for (int k = 0; k < kBlocks; ++k) {
+        uint32_t r[4];
+        ldsm4t(r, at + k * 32);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          mma16816(o[nt][k], r[0], r[1], r[2], r[3], ph[nt][0], ph[nt][1]);
+          mma16816(o[nt][k], r[0], r[1], r[2], r[3], pl[nt][0], pl[nt][1]);
+        }
+      }
+    } else {
+      const uint32_t at = vt + ((lane & 7) + (lane & 8)) * S::kPitch;
+#pragma unroll
+      for (int k = 0; k < kBlocks; k += 2) {
+        uint32_t r[4];
+        if (k + 1 < kBlocks) ldsm4t(r, at + k * 16 + (lane >> 4) * 16);
+        else ldsm2t(r[0], r[1], at + k * 16);
+#pragma unroll
+        for (int u = 0; u < 2 && k + u < kBlocks; ++u) {
+          // bytes: token 2c dims 2g, 2g + 1, token 2c + 1 the same; paired by dim
+          const uint32_t lo = __byte_perm(r[2 * u], 0, 0x3120);
+          const uint32_t hi = __byte_perm(r[2 * u + 1], 0, 0x3120);
+          const uint32_t a0 = widen(lo), a1 = widen(lo >> 16), a2 = widen(hi), a3 = widen(hi >> 16);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            mma_f16(o[nt][k + u], a0, a1, a2, a3, ph[nt][0], ph[nt][1]);
+        }
+      }
+    }
+  };
+
+  auto sum_l = [&]() {  // the lanes' shares of the sums of weights
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], d);
+  };
+  auto store_slot = [&](float* dst) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int k = 0; k < kBlocks; ++k)
+        reinterpret_cast<float4*>(dst)[(nt * kBlocks + k) * 32 + lane] =
+            make_float4(o[nt][k][0], o[nt][k][1], o[nt][k][2], o[nt][k][3]);
+      if (lane < 4) {
+        dst[S::kOut + nt * 8 + 2 * lane] = m[nt][0];
+        dst[S::kOut + nt * 8 + 2 * lane + 1] = m[nt][1];
+        dst[S::kOut + NT * 8 + nt * 8 + 2 * lane] = l[nt][0];
+        dst[S::kOut + NT * 8 + nt * 8 + 2 * lane + 1] = l[nt][1];
+      }
+    }
+  };
+
+  // ---- the run
+  int tail = 0;  // 1: a partial segment is left in registers, 2: it has the first tile, 4: the last
+  if (count > 0) {
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) load(i);
+    int stage = 0, free_stage = kStages - 1;
+    for (int i = 0; i < count; ++i) {
+      cp_wait<kStages - 2>();
+      __syncwarp();
+      load(free_stage);
+      const int4 info = s_info[warp][stage];
+      if (!open) {
+        open = true;
+        from_start = i > 0 || s_begin[warp].z == 0;
+        begin_segment(info.x, info.y);
+        seg_end = begin + i + info.w;
+      }
+      if (info.z > 0) tile(stage, info.z);
+      free_stage = stage;
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+      const bool done = info.w == 1;
+      if (done || i + 1 == count) {
+        sum_l();
+        open = false;
+        if (done && from_start) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const float i0 = R::inverse(a, shc, l[nt][0]), i1 = R::inverse(a, shc, l[nt][1]);
+#pragma unroll
+            for (int k = 0; k < kBlocks; ++k)
+              R::store(a, sb, shc, nt, k,
+                       make_float4(o[nt][k][0], o[nt][k][1], o[nt][k][2], o[nt][k][3]), i0, i1,
+                       lane);
+            R::store_lse(a, sb, shc, nt, m[nt][0], l[nt][0], m[nt][1], l[nt][1], lane);
+          }
+        } else if (i + 1 < count) {
+          store_slot(a.ws + slot_of(worker, 1) * S::kSlot);
+        } else {
+          tail = 1 | (from_start ? 2 : 0) | (done ? 4 : 0);
+        }
+      }
+    }
+    cp_wait<0>();
+    __syncwarp();
+    if (tail) store_slot(reinterpret_cast<float*>(ring));
+  }
+  if (lane == 0) {
+    s_tail[warp] = make_int4(tail, sb, shc, 0);
+    Split sp{-1, 0, 0, 0};
+    if ((tail & 3) == 3) {  // its last tile's worker: the largest w with w * total / workers <= it
+      const int64_t last = (seg_end * workers + total - 1) / total - 1;
+      sp = Split{sb, shc, static_cast<int32_t>(last), (last + 1) * total / workers > seg_end};
+    }
+    s_split[warp] = sp;
+  }
+  __syncthreads();
+
+  // ---- join the tails of this CTA: a run of warps from one that is not continued from its
+  // left neighbour to the last one that continues it
+  for (int w0 = 0; w0 < kWarps; ++w0) {
+    const int4 head = s_tail[w0];
+    if (!(head.x & 1) || (w0 > 0 && !(head.x & 2))) continue;
+    int w1 = w0;
+    while (w1 + 1 < kWarps && (s_tail[w1 + 1].x & 3) == 1) ++w1;
+    const bool whole = (head.x & 2) && (s_tail[w1].x & 4);
+    float* const slot = a.ws + slot_of(first_worker + w0, 0) * S::kSlot;
+    for (int at = warp; at < NT * kBlocks; at += kWarps) {
+      const int nt = at / kBlocks, k = at % kBlocks;
+      float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      auto part = [&](int w) {
+        return reinterpret_cast<const float*>(ring_mem + static_cast<size_t>(w) * kStages * S::kTileBytes);
+      };
+      for (int w = w0; w <= w1; ++w)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) top[j] = fmaxf(top[j], part(w)[S::kOut + nt * 8 + 2 * c + j]);
+      for (int w = w0; w <= w1; ++w) {
+        const float* p = part(w);
+        const float x0 = weight_of(p[S::kOut + nt * 8 + 2 * c], top[0]);
+        const float x1 = weight_of(p[S::kOut + nt * 8 + 2 * c + 1], top[1]);
+        const float4 v = reinterpret_cast<const float4*>(p)[at * 32 + lane];
+        sum[0] += x0 * p[S::kOut + NT * 8 + nt * 8 + 2 * c];
+        sum[1] += x1 * p[S::kOut + NT * 8 + nt * 8 + 2 * c + 1];
+        acc.x += x0 * v.x;
+        acc.y += x1 * v.y;
+        acc.z += x0 * v.z;
+        acc.w += x1 * v.w;
+      }
+      if (whole) {
+        R::store(a, head.y, head.z, nt, k, acc, R::inverse(a, head.z, sum[0]),
+                 R::inverse(a, head.z, sum[1]), lane);
+        if (k == 0) R::store_lse(a, head.y, head.z, nt, top[0], sum[0], top[1], sum[1], lane);
+      } else {
+        reinterpret_cast<float4*>(slot)[at * 32 + lane] = acc;
+        if (k == 0 && lane < 4) {
+          slot[S::kOut + nt * 8 + 2 * lane] = top[0];
+          slot[S::kOut + nt * 8 + 2 * lane + 1] = top[1];
+          slot[S::kOut + NT * 8 + nt * 8 + 2 * lane] = sum[0];
+          slot[S::kOut + NT * 8 + nt * 8 + 2 * lane + 1] = sum[1];
+        }
+      }
+    }
+    if (whole && threadIdx.x == 0) s_split[w0].b = -1;
+  }
+  __syncthreads();
+  Split* const splits =
+      reinterpret_cast<Split*>(a.ws + slot_of(static_cast<int64_t>(gridDim.x) * kWarps, 0) * S::kSlot);
+  if (threadIdx.x < kWarps) splits[first_worker + threadIdx.x] = s_split[threadIdx.x];
 }
 
+// Joins the partial results of the segments that cross CTAs: one CTA for each worker at
+// which such a segment begins.
+template <int D, bool kE4m3, int NT>
+__global__ void __launch_bounds__(128) paged_join_kernel(PagedArgs a) {
+  using S = Shape<D, kE4m3, NT>;
+  using R = Rows<D, kE4m3, NT>;
+  constexpr int kWarps = S::kWarps;
+  allow_dependent_launch();
+  wait_prerequisite();
+  const int64_t w0 = blockIdx.x;
+  const Split sp = reinterpret_cast<const Split*>(a.ws + slot_of(gridDim.x, 0) * S::kSlot)[w0];
+  if (sp.b < 0) return;
+  const int lane = threadIdx.x & 31, c = lane & 3;
+  // parts in line order: the tail slot of w0, the tail slots of the first workers of the
+  // CTAs behind it, the head slot of the last worker if its run goes on
+  const int64_t last_tail = sp.last - sp.head;
+  const int mid = static_cast<int>(last_tail / kWarps - w0 / kWarps);  // >= 0: last_tail >= w0
+  const int parts = 1 + mid + sp.head;
+  auto part = [&](int i) -> const float* {
+    const int64_t s = i == 0 ? slot_of(w0, 0)
+                      : i <= mid ? slot_of((w0 / kWarps + i) * kWarps, 0)
+                                 : slot_of(sp.last, 1);
+    return a.ws + s * S::kSlot;
+  };
+  for (int at = threadIdx.x >> 5; at < NT * S::kBlocks; at += 4) {
+    const int nt = at / S::kBlocks, k = at % S::kBlocks;
+    float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int i = 0; i < parts; ++i) {
+      const float2 x = *reinterpret_cast<const float2*>(part(i) + S::kOut + nt * 8 + 2 * c);
+      top[0] = fmaxf(top[0], x.x);
+      top[1] = fmaxf(top[1], x.y);
+    }
+#pragma unroll 4
+    for (int i = 0; i < parts; ++i) {
+      const float* p = part(i);
+      const float2 x = *reinterpret_cast<const float2*>(p + S::kOut + nt * 8 + 2 * c);
+      const float2 y = *reinterpret_cast<const float2*>(p + S::kOut + NT * 8 + nt * 8 + 2 * c);
+      const float4 v = reinterpret_cast<const float4*>(p)[at * 32 + lane];
+      const float x0 = weight_of(x.x, top[0]), x1 = weight_of(x.y, top[1]);
+      sum[0] += x0 * y.x;
+      sum[1] += x1 * y.y;
+      acc.x += x0 * v.x;
+      acc.y += x1 * v.y;
+      acc.z += x0 * v.z;
+      acc.w += x1 * v.w;
+    }
+    R::store(a, sp.b, sp.hc, nt, k, acc, R::inverse(a, sp.hc, sum[0]),
+             R::inverse(a, sp.hc, sum[1]), lane);
+    if (k == 0) R::store_lse(a, sp.b, sp.hc, nt, top[0], sum[0], top[1], sum[1], lane);
+  }
+}
+
+// CTAs of the main kernel: one per SM, fewer where the longest possible line is shorter.
+template <int D, bool kE4m3, int NT>
+int64_t grid_of(const PagedArgs& a) {
+  using S = Shape<D, kE4m3, NT>;
+  const int64_t tiles = (a.max_len + kTile - 1) / kTile * a.batch * a.hkv * a.chunks;
+  int64_t ctas = std::min<int64_t>(sm_count(), kMaxWorkers / S::kWarps);
+  return std::max<int64_t>(1, std::min(ctas, (tiles + S::kWarps - 1) / S::kWarps));
+}
+
+template <int D, bool kE4m3, int NT>
+void launch(PagedArgs a, cudaStream_t st) {
+  using S = Shape<D, kE4m3, NT>;
+  a.chunks = (a.group + 8 * NT - 1) / (8 * NT);
+  static std::once_flag once[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::call_once(once[dev & 63], [] {
+    cudaFuncSetAttribute(paged_attn_kernel<D, kE4m3, NT>,
+                         cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::kSmem));
+    cudaFuncSetAttribute(paged_join_kernel<D, kE4m3, NT>,
+                         cudaFuncAttributePreferredSharedMemoryCarveout,
+                         cudaSharedmemCarveoutMaxShared);
+  });
+  const unsigned ctas = static_cast<unsigned>(grid_of<D, kE4m3, NT>(a));
+  launch_pdl(paged_attn_kernel<D, kE4m3, NT>, dim3(ctas), dim3(S::kWarps * 32), S::kSmem, st, a);
+  launch_pdl(paged_join_kernel<D, kE4m3, NT>, dim3(ctas * S::kWarps), dim3(128), 0, st, a);
+}
+
+// Up to 8 query heads per KV head use one column tile; wider groups two, which halves the
+// K and V traffic of their segments (head_dim 256 keeps one: its accumulators of two would
+// not fit the registers).
 template <int D>
 void launch_d(const PagedArgs& a, bool e4m3, cudaStream_t st) {
-  const dim3 grid(static_cast<unsigned>(a.batch) * a.hq);
-  if (e4m3) launch_pdl(paged_attn_kernel<D, true>, grid, dim3(32), 0, st, a);
-  else launch_pdl(paged_attn_kernel<D, false>, grid, dim3(32), 0, st, a);
+  if constexpr (D <= 128) {
+    if (a.group > 8) {
+      if (e4m3) launch<D, true, 2>(a, st);
+      else launch<D, false, 2>(a, st);
+      return;
+    }
+  }
+  if (e4m3) launch<D, true, 1>(a, st);
+  else launch<D, false, 1>(a, st);
 }
 
 }  // namespace
@@ -99,7 +774,14 @@ void launch_d(const PagedArgs& a, bool e4m3, cudaStream_t st) {
 
 using namespace umic;
 
-extern "C" size_t umic_paged_attention_workspace_bytes(int32_t, int32_t, int32_t) { return 16; }
+extern "C" size_t umic_paged_attention_workspace_bytes(int32_t hq, int32_t hkv,
+                                                       int32_t head_dim) {
+  if (hq <= 0 || hkv <= 0 || head_dim <= 0) return 0;
+  // per warp: two partial results (O, m, l of its query heads) and a split record
+  const size_t heads = hq / hkv > 8 && head_dim <= 128 ? 16 : 8;
+  const size_t workers = static_cast<size_t>(std::min<int64_t>(sm_count() * 8, kMaxWorkers));
+  return workers * (2 * heads * (head_dim + 2) * sizeof(float) + sizeof(Split));
+}
 
 extern "C" int umic_paged_attention(
     const void* q, int64_t q_sb, int64_t q_sh, const void* k_pages, const void* v_pages,
@@ -144,11 +826,27 @@ extern "C" int umic_paged_attention(
   uint32_t* err = device_error_word();
   if (!err) return fail(UMIC_ERR_DEVICE, "%s: no device error word", me);
   const bool e4m3 = cache_dtype == UMIC_DTYPE_E4M3;
-  PagedArgs a{static_cast<const __nv_bfloat16*>(q), k_pages, v_pages, e4m3 ? k_scale : nullptr,
-              e4m3 ? v_scale : nullptr, block_table, kv_lens,
-              static_cast<__nv_bfloat16*>(out), lse, err, q_sb, q_sh, pg_sp, pg_sh, pg_ss,
-              table_stride, max_pages * page_size, num_pages, o_sb, o_sh,
-              static_cast<int32_t>(page_size), hq, hkv, static_cast<int32_t>(batch), scale};
+  const int64_t es = e4m3 ? 1 : 2;
+  PagedArgs a{};
+  a.q = static_cast<const __nv_bfloat16*>(q);
+  a.k_pages = static_cast<const char*>(k_pages);
+  a.v_pages = static_cast<const char*>(v_pages);
+  a.k_scale = e4m3 ? k_scale : nullptr;
+  a.v_scale = e4m3 ? v_scale : nullptr;
+  a.table = block_table;
+  a.lens = kv_lens;
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.lse = lse;
+  a.err = err;
+  a.ws = static_cast<float*>(workspace);
+  a.q_sb = q_sb; a.q_sh = q_sh; a.o_sb = o_sb; a.o_sh = o_sh;
+  a.pg_sp = pg_sp * es; a.pg_sh = pg_sh * es; a.pg_ss = pg_ss * es;
+  a.table_stride = table_stride;
+  a.max_len = max_pages * page_size;
+  a.num_pages = num_pages;
+  a.page_size = static_cast<int32_t>(page_size);
+  a.hq = hq; a.hkv = hkv; a.batch = static_cast<int32_t>(batch); a.group = hq / hkv;
+  a.scale_log2 = scale * 1.4426950408889634f;
   cudaStream_t st = as_stream(stream);
   if (head_dim == 64) launch_d<64>(a, e4m3, st);
   else if (head_dim == 80) launch_d<80>(a, e4m3, st);
