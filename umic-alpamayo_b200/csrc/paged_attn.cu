@@ -7,7 +7,7 @@
 // all that matters is to keep its loads in flight.
 //
 // Work. A segment is one request's one KV head (up to 8 * NT query heads; wider groups are
-// cut into several segments), a tile 16 of its tokens. All tiles of all segments form one
+// cut into several segments), a tile 16 or 32 of its tokens. All tiles of all segments form one
 // line, and every warp takes an equal run of it, whatever the lengths: no warp idles
 // because its request is short. A warp needs no other: it copies its tiles into its own
 // ring with 16-byte asynchronous loads, kStages ahead across segment borders, and waits for
@@ -39,7 +39,7 @@
 namespace umic {
 namespace {
 
-constexpr int kTile = 16;             // tokens per tile
+constexpr int kSub = 16;              // tokens per subtile: rows of one mma, within one page
 constexpr float kF16Shift = 14.f;     // e4m3 path: weights are held as 2^14 p
 constexpr int kSmemBudget = 216 * 1024;
 constexpr int64_t kMaxWorkers = 2048;  // warps of the main kernel, bounds the workspace
@@ -54,8 +54,8 @@ struct PagedArgs {
   uint32_t* err;
   float* ws;
   int64_t q_sb, q_sh, pg_sp, pg_sh, pg_ss;  // pg_* in bytes
-  int64_t table_stride, max_len, num_pages, o_sb, o_sh;
-  int32_t page_size, hq, hkv, batch, group, chunks;  // chunks: segments per KV head
+  int64_t table_stride, num_pages, o_sb, o_sh;
+  int32_t max_len, page_size, hq, hkv, batch, group, chunks;  // chunks: segments per KV head
   float scale_log2;
 };
 
@@ -65,7 +65,12 @@ struct Shape {
   static constexpr int kRow = D * (kE4m3 ? 1 : 2);                   // bytes of a token's row
   static constexpr int kPitch = kRow + ((kRow / 16) % 2 ? 0 : 16);  // odd count of 16 B: no
                                                                     // bank conflicts
-  static constexpr int kTileBytes = 2 * kTile * kPitch;             // K, then V
+  // Rows of up to 192 bytes go two subtiles a tile: the running maximum and its shuffles
+  // cost a tile the same whatever it holds.
+  static constexpr int MT = kRow <= 192 ? 2 : 1;
+  static constexpr int kTile = kSub * MT;                           // tokens per tile
+  static constexpr int kSubBytes = 2 * kSub * kPitch;               // K, then V
+  static constexpr int kTileBytes = MT * kSubBytes;
   static constexpr int kWarps = D == 256 && !kE4m3 ? 4 : 8;
   static constexpr int kFit = kSmemBudget / (kWarps * kTileBytes);
   static constexpr int kStages = kFit < 6 ? kFit : 6;
@@ -157,10 +162,21 @@ __device__ __forceinline__ uint32_t widen(uint32_t two) {
   return static_cast<uint32_t>(h.x) | static_cast<uint32_t>(h.y) << 16;
 }
 
-__device__ __forceinline__ int64_t clamped_len(const PagedArgs& a, int b) {
-  const int64_t n = a.lens[b];
-  return n < 0 ? 0 : n > a.max_len ? a.max_len : n;
+__device__ __forceinline__ int clamped_len(const PagedArgs& a, int b) {
+  return max(0, min(a.lens[b], a.max_len));
 }
+
+// The line of `total` tiles cut into `workers` runs, the first `longer` one tile longer.
+// (32-bit: a 64-bit division takes hundreds of cycles here.)
+struct Line {
+  int base, longer;
+  __device__ Line(int total, int workers) : base(total / workers), longer(total % workers) {}
+  __device__ int begin(int w) const { return w * base + min(w, longer); }
+  __device__ int worker_of(int x) const {
+    const int cut = longer * (base + 1);
+    return x < cut ? x / (base + 1) : longer + (x - cut) / base;
+  }
+};
 
 // One warp's view of a segment's rows: where the outputs of its heads go.
 template <int D, bool kE4m3, int NT>
@@ -221,11 +237,14 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
   using S = Shape<D, kE4m3, NT>;
   using R = Rows<D, kE4m3, NT>;
   constexpr int kWarps = S::kWarps, kStages = S::kStages, kBlocks = S::kBlocks;
-  constexpr int kThreads = kWarps * 32;
+  constexpr int kThreads = kWarps * 32, MT = S::MT, kTile = S::kTile;
+  auto tiles_of = [](int len) { return (len + kTile - 1) / kTile; };
   extern __shared__ __align__(16) char ring_mem[];
-  __shared__ int4 s_info[kWarps][kStages];  // request, segment, valid rows, tiles left
-  __shared__ int4 s_begin[kWarps];          // request, segment, tile at a warp's start
-  __shared__ int64_t s_warp_sum[kWarps];
+  __shared__ int4 s_info[kWarps][kStages];  // request, segment, valid rows (a byte per
+                                            // subtile), tiles left of the segment
+  __shared__ int4 s_begin[kWarps];          // request, segment, tile and request length at a
+                                            // warp's start
+  __shared__ int s_warp_sum[kWarps];
   __shared__ int4 s_tail[kWarps];  // has a tail | 2 starts it | 4 ends it, request, segment
   __shared__ Split s_split[kWarps];
 
@@ -237,40 +256,47 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
   // ---- the line of tiles, and where each warp's run begins on it
   const int per = (a.batch + kThreads - 1) / kThreads;
   const int b0 = min(a.batch, static_cast<int>(threadIdx.x) * per), b1 = min(a.batch, b0 + per);
-  int64_t mine = 0;
+  int mine = 0, first_len = 0;
   for (int b = b0; b < b1; ++b) {
-    const int64_t n = a.lens[b];
+    const int n = a.lens[b];
     if (blockIdx.x == 0 && (n < 0 || n > a.max_len)) atomicOr(a.err, UMIC_DEVERR_BAD_PAGE);
-    mine += (clamped_len(a, b) + kTile - 1) / kTile;
+    const int len = max(0, min(n, a.max_len));
+    if (b == b0) first_len = len;
+    mine += tiles_of(len);
   }
-  int64_t upto = mine;
+  int upto = mine;
+#pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+    const int x = __shfl_up_sync(0xffffffffu, upto, o);
     if (lane >= o) upto += x;
   }
   if (lane == 31) s_warp_sum[warp] = upto;
   __syncthreads();
-  int64_t total = 0;
+  int total = 0;
   upto -= mine;
+#pragma unroll
   for (int w = 0; w < kWarps; ++w) {
     if (w == warp) upto += total;
     total += s_warp_sum[w];
   }
   total *= hcs;
-  const int64_t workers = min(static_cast<int64_t>(gridDim.x) * kWarps, total);
-  const int64_t first_worker = static_cast<int64_t>(blockIdx.x) * kWarps;
-  for (int w = 0; w < kWarps && first_worker + w < workers; ++w) {
-    const int64_t at = (first_worker + w) * total / workers;
-    if (at < upto * hcs || at >= (upto + mine) * hcs) continue;
-    int64_t from = upto * hcs;
-    for (int b = b0; b < b1; ++b) {
-      const int64_t tiles = (clamped_len(a, b) + kTile - 1) / kTile;
-      if (at < from + tiles * hcs) {
-        s_begin[w] = make_int4(b, static_cast<int>((at - from) / tiles),
-                               static_cast<int>((at - from) % tiles), 0);
-        break;
+  const int workers = min(static_cast<int>(gridDim.x) * kWarps, total);
+  const int first_worker = static_cast<int>(blockIdx.x) * kWarps;
+  const Line line(total, max(workers, 1));
+  if (mine > 0 && first_worker < workers &&
+      line.begin(first_worker + kWarps) > upto * hcs) {
+    for (int w = 0; w < kWarps && first_worker + w < workers; ++w) {
+      int at = line.begin(first_worker + w) - upto * hcs;
+      if (at < 0 || at >= mine * hcs) continue;
+      int len = first_len;
+      for (int b = b0;; len = clamped_len(a, ++b)) {
+        const int tiles = tiles_of(len);
+        if (at < tiles * hcs) {
+          s_begin[w] = make_int4(b, at / tiles, at % tiles, len);
+          break;
+        }
+        at -= tiles * hcs;
       }
-      from += tiles * hcs;
     }
   }
   // requests without tokens: zeros
@@ -284,68 +310,99 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
   }
   __syncthreads();
 
-  const int64_t worker = first_worker + warp;
-  const int64_t begin = worker < workers ? worker * total / workers : 0;
-  const int64_t end = worker < workers ? (worker + 1) * total / workers : 0;
-  const int count = static_cast<int>(end - begin);
+  const int worker = first_worker + warp;
+  const int begin = line.begin(worker);
+  const int count = worker < workers ? line.begin(worker + 1) - begin : 0;
   char* const ring = ring_mem + static_cast<size_t>(warp) * kStages * S::kTileBytes;
   const uint32_t ring_addr = smem_addr(ring);
 
-  // ---- loader: the next tile to copy
-  int lb = 0, lhc = 0, lt = 0, ltiles = 0, lpi = 0, loff = 0;
-  int64_t llen = 0;
-  int32_t lpage = 0;
+  // ---- loader: the next tile to copy. Pages are looked up one tile ahead of their copies.
+  int lb = 0, lhc = 0, lt = 0, ltiles = 0, lpi = 0, loff = 0, llen = 0;
+  int page_id[MT], page_off[MT];
+  const int32_t* row_of_table = a.table;
+  auto look_up = [&]() {  // pages of tile lt; steps (lpi, loff) behind it
+#pragma unroll
+    for (int u = 0; u < MT; ++u) {
+      page_off[u] = loff;
+      page_id[u] = u == 0 || lt * kTile + u * kSub < llen ? row_of_table[lpi] : 0;
+      if ((loff += kSub) == a.page_size) {
+        loff = 0;
+        ++lpi;
+      }
+    }
+  };
   if (count > 0) {
     const int4 st = s_begin[warp];
     lb = st.x;
     lhc = st.y;
     lt = st.z;
-    llen = clamped_len(a, lb);
-    ltiles = static_cast<int>((llen + kTile - 1) / kTile);
+    llen = st.w;
+    ltiles = tiles_of(llen);
+    row_of_table += lb * a.table_stride;
     lpi = lt * kTile / a.page_size;
-    loff = lt * kTile % a.page_size;
-    lpage = a.table[lb * a.table_stride + lpi];
+    loff = lt * kTile - lpi * a.page_size;
+    look_up();
   }
+  constexpr int kCols = S::kRow / 16;  // 16-byte pieces of a row
+  constexpr int kCopies = (kSub * kCols + 31) / 32;
+  const bool dense = a.pg_ss == S::kRow;  // a page's rows of a head lie one behind the other
+  const int64_t v_minus_k = a.v_pages - a.k_pages;
   int loaded = 0;
   auto load = [&](int stage) {
     if (loaded < count) {
       ++loaded;
-      int rows = static_cast<int>(min(static_cast<int64_t>(kTile), llen - static_cast<int64_t>(lt) * kTile));
-      int64_t page = lpage;
-      if (page < 0 || page >= a.num_pages) {
-        if (lane == 0) atomicOr(a.err, UMIC_DEVERR_BAD_PAGE);
-        page = 0;
-        rows = 0;
-      }
-      if (lane == 0) s_info[warp][stage] = make_int4(lb, lhc, rows, ltiles - lt);
-      const int64_t base = page * a.pg_sp + lhc / a.chunks * a.pg_sh + loff * a.pg_ss;
-      const uint32_t dst = ring_addr + stage * S::kTileBytes;
-      constexpr int kCols = S::kRow / 16;  // 16-byte pieces of a row
+      int rows_of = 0;
+      const int64_t head_at = lhc / a.chunks * a.pg_sh;
 #pragma unroll
-      for (int i = 0; i < (kTile * kCols + 31) / 32; ++i) {
-        const int x = i * 32 + lane, row = x / kCols, col = x % kCols;
-        if ((kTile * kCols) % 32 != 0 && row >= kTile) break;
-        // rows behind the length are filled with zeros: a weight of 0 times what an
-        // unwritten page holds could be NaN
-        const bool there = row < rows;
-        const int64_t at = base + (there ? row * a.pg_ss + col * 16 : 0);
-        cp_async16(dst + row * S::kPitch + col * 16, a.k_pages + at, there);
-        cp_async16(dst + kTile * S::kPitch + row * S::kPitch + col * 16, a.v_pages + at, there);
+      for (int u = 0; u < MT; ++u) {
+        int rows = max(0, min(kSub, llen - lt * kTile - u * kSub));
+        int64_t page = page_id[u];
+        if (page < 0 || page >= a.num_pages) {
+          if (lane == 0 && rows > 0) atomicOr(a.err, UMIC_DEVERR_BAD_PAGE);
+          page = 0;
+          rows = 0;
+        }
+        rows_of |= rows << (8 * u);
+        const char* k = a.k_pages + page * a.pg_sp + head_at + page_off[u] * a.pg_ss;
+        const uint32_t dst = ring_addr + stage * S::kTileBytes + u * S::kSubBytes;
+        if (dense && rows == kSub) {
+          k += lane * 16;
+          const char* v = k + v_minus_k;
+#pragma unroll
+          for (int i = 0; i < kCopies; ++i) {
+            const int x = i * 32 + lane;
+            const uint32_t to = dst + x / kCols * S::kPitch + x % kCols * 16;
+            if ((kSub * kCols) % 32 != 0 && x >= kSub * kCols) break;
+            cp_async16(to, k + i * 512, true);
+            cp_async16(to + kSub * S::kPitch, v + i * 512, true);
+          }
+        } else {
+          // rows behind the length are filled with zeros: a weight of 0 times what an
+          // unwritten page holds could be NaN
+#pragma unroll
+          for (int i = 0; i < kCopies; ++i) {
+            const int x = i * 32 + lane, row = x / kCols;
+            const uint32_t to = dst + row * S::kPitch + x % kCols * 16;
+            if ((kSub * kCols) % 32 != 0 && x >= kSub * kCols) break;
+            const char* at = k + row * a.pg_ss + x % kCols * 16;
+            cp_async16(to, at, row < rows);
+            cp_async16(to + kSub * S::kPitch, at + v_minus_k, row < rows);
+          }
+        }
       }
-      if (loaded < count) {  // step on; the page is fetched now and used by the next call
+      if (lane == 0) s_info[warp][stage] = make_int4(lb, lhc, rows_of, ltiles - lt);
+      if (loaded < count) {
         if (++lt == ltiles) {
           lt = lpi = loff = 0;
           if (++lhc == hcs) {
             lhc = 0;
             do llen = clamped_len(a, ++lb);
             while (llen == 0);
-            ltiles = static_cast<int>((llen + kTile - 1) / kTile);
+            ltiles = tiles_of(llen);
+            row_of_table = a.table + lb * a.table_stride;
           }
-          lpage = a.table[lb * a.table_stride];
-        } else if ((loff += kTile) == a.page_size) {
-          loff = 0;
-          lpage = a.table[lb * a.table_stride + ++lpi];
         }
+        look_up();
       }
     }
     cp_commit();
@@ -358,7 +415,7 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
   float m[NT][2], l[NT][2], fac[NT][2];
   int sb = 0, shc = 0;
   bool open = false, from_start = false;
-  int64_t seg_end = 0;  // line position behind the segment
+  int seg_end = 0;  // line position behind the segment
 
   auto begin_segment = [&](int b, int hc) {
     sb = b;
@@ -415,54 +472,64 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
     }
   };
 
-  auto tile = [&](int stage, int rows) {
-    const uint32_t kt = ring_addr + stage * S::kTileBytes, vt = kt + kTile * S::kPitch;
+  auto tile = [&](int stage, int rows_of) {
+    const uint32_t at0 = ring_addr + stage * S::kTileBytes;
+    // S^T: one accumulator per subtile, or two that share the chain of a single one
     float s[NT][2][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int j = 0; j < 4; ++j) s[nt][0][j] = s[nt][1][j] = 0.f;
-    // two accumulators: half the chain of dependent products
-    if constexpr (!kE4m3) {
-      const uint32_t at = kt + ((lane & 7) + (lane & 8)) * S::kPitch + (lane >> 4) * 16;
+    const uint32_t k_at = at0 + ((lane & 7) + (lane & 8)) * S::kPitch + (lane >> 4) * 16;
 #pragma unroll
-      for (int k = 0; k < kBlocks; ++k) {
-        uint32_t r[4];
-        ldsm4(r, at + k * 32);
+    for (int u = 0; u < MT; ++u) {
+      const uint32_t at = k_at + u * S::kSubBytes;
+      if constexpr (!kE4m3) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          mma16816(s[nt][k & 1], r[0], r[1], r[2], r[3], qf[nt][k][0], qf[nt][k][1]);
-      }
-    } else {
-      const uint32_t at = kt + ((lane & 7) + (lane & 8)) * S::kPitch;
-#pragma unroll
-      for (int k = 0; k < kBlocks; k += 2) {
-        uint32_t r[4];
-        if (k + 1 < kBlocks) ldsm4(r, at + k * 16 + (lane >> 4) * 16);
-        else ldsm2(r[0], r[1], at + k * 16);
-#pragma unroll
-        for (int u = 0; u < 2 && k + u < kBlocks; ++u) {
-          const uint32_t a0 = widen(r[2 * u]), a1 = widen(r[2 * u + 1]);
-          const uint32_t a2 = widen(r[2 * u] >> 16), a3 = widen(r[2 * u + 1] >> 16);
+        for (int k = 0; k < kBlocks; ++k) {
+          uint32_t r[4];
+          ldsm4(r, at + k * 32);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
-            mma_f16(s[nt][u], a0, a1, a2, a3, qf[nt][k + u][0], qf[nt][k + u][1]);
+            mma16816(s[nt][MT == 2 ? u : k & 1], r[0], r[1], r[2], r[3], qf[nt][k][0],
+                     qf[nt][k][1]);
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < kBlocks; k += 2) {
+          uint32_t r[4];
+          if (k + 1 < kBlocks) ldsm4(r, at + k * 16);
+          else ldsm2(r[0], r[1], at + k * 16);
+#pragma unroll
+          for (int x = 0; x < 2 && k + x < kBlocks; ++x) {
+            const uint32_t a0 = widen(r[2 * x]), a1 = widen(r[2 * x + 1]);
+            const uint32_t a2 = widen(r[2 * x] >> 16), a3 = widen(r[2 * x + 1] >> 16);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              mma_f16(s[nt][MT == 2 ? u : x], a0, a1, a2, a3, qf[nt][k + x][0], qf[nt][k + x][1]);
+          }
         }
       }
     }
-    uint32_t ph[NT][2], pl[NT][2];
+    uint32_t ph[NT][MT][2], pl[NT][MT][2];
     bool moved = false;
     float keep[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      float x[4];
+      float x[MT][4], top[2] = {m[nt][0], m[nt][1]};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = (s[nt][0][j] + s[nt][1][j]) * fac[nt][j & 1];
-      if (rows < kTile) {
-        if (g >= rows) x[0] = x[1] = -INFINITY;
-        if (g + 8 >= rows) x[2] = x[3] = -INFINITY;
+      for (int u = 0; u < MT; ++u) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          x[u][j] = (MT == 2 ? s[nt][u][j] : s[nt][0][j] + s[nt][1][j]) * fac[nt][j & 1];
+        const int rows = rows_of >> (8 * u) & 255;
+        if (rows < kSub) {
+          if (g >= rows) x[u][0] = x[u][1] = -INFINITY;
+          if (g + 8 >= rows) x[u][2] = x[u][3] = -INFINITY;
+        }
+        top[0] = fmaxf(top[0], fmaxf(x[u][0], x[u][2]));
+        top[1] = fmaxf(top[1], fmaxf(x[u][1], x[u][3]));
       }
-      float top[2] = {fmaxf(x[0], x[2]), fmaxf(x[1], x[3])};
 #pragma unroll
       for (int d = 4; d < 32; d <<= 1) {
         top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], d));
@@ -471,29 +538,32 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
       float ref[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        top[j] = fmaxf(top[j], m[nt][j]);
         ref[j] = top[j] == -INFINITY ? 0.f : top[j];
         keep[nt][j] = exp2_fast(m[nt][j] - ref[j]);
         moved |= keep[nt][j] != 1.f;
         m[nt][j] = top[j];
+        l[nt][j] *= keep[nt][j];
         if constexpr (kE4m3) ref[j] -= kF16Shift;
       }
-      float p[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) p[j] = exp2_fast(x[j] - ref[j & 1]);
-      l[nt][0] = l[nt][0] * keep[nt][0] + (p[0] + p[2]);
-      l[nt][1] = l[nt][1] * keep[nt][1] + (p[1] + p[3]);
-      if constexpr (kE4m3) {
-        ph[nt][0] = transpose8x8(pack_f16(p[0], p[1]));
-        ph[nt][1] = transpose8x8(pack_f16(p[2], p[3]));
-      } else {
-        const uint32_t h0 = pack_bf16(p[0], p[1]), h1 = pack_bf16(p[2], p[3]);
-        ph[nt][0] = transpose8x8(h0);
-        ph[nt][1] = transpose8x8(h1);
-        pl[nt][0] = transpose8x8(pack_bf16(p[0] - __uint_as_float(h0 << 16),
-                                           p[1] - __uint_as_float(h0 & 0xffff0000u)));
-        pl[nt][1] = transpose8x8(pack_bf16(p[2] - __uint_as_float(h1 << 16),
-                                           p[3] - __uint_as_float(h1 & 0xffff0000u)));
+      for (int u = 0; u < MT; ++u) {
+        float p[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p[j] = exp2_fast(x[u][j] - ref[j & 1]);
+        l[nt][0] += p[0] + p[2];
+        l[nt][1] += p[1] + p[3];
+        if constexpr (kE4m3) {
+          ph[nt][u][0] = transpose8x8(pack_f16(p[0], p[1]));
+          ph[nt][u][1] = transpose8x8(pack_f16(p[2], p[3]));
+        } else {
+          const uint32_t h0 = pack_bf16(p[0], p[1]), h1 = pack_bf16(p[2], p[3]);
+          ph[nt][u][0] = transpose8x8(h0);
+          ph[nt][u][1] = transpose8x8(h1);
+          pl[nt][u][0] = transpose8x8(pack_bf16(p[0] - __uint_as_float(h0 << 16),
+                                                p[1] - __uint_as_float(h0 & 0xffff0000u)));
+          pl[nt][u][1] = transpose8x8(pack_bf16(p[2] - __uint_as_float(h1 << 16),
+                                                p[3] - __uint_as_float(h1 & 0xffff0000u)));
+        }
       }
     }
     if (__any_sync(0xffffffffu, moved)) {
@@ -504,34 +574,40 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
 #pragma unroll
           for (int j = 0; j < 4; ++j) o[nt][k][j] *= keep[nt][j & 1];
     }
-    if constexpr (!kE4m3) {
-      const uint32_t at = vt + ((lane & 7) + ((lane >> 4) << 3)) * S::kPitch + ((lane >> 3) & 1) * 16;
 #pragma unroll
-      for (int k = 0; k < kBlocks; ++k) {
-        uint32_t r[4];
-        ldsm4t(r, at + k * 32);
+    for (int u = 0; u < MT; ++u) {
+      const uint32_t vt = at0 + u * S::kSubBytes + kSub * S::kPitch;
+      if constexpr (!kE4m3) {
+        const uint32_t at =
+            vt + ((lane & 7) + ((lane >> 4) << 3)) * S::kPitch + ((lane >> 3) & 1) * 16;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          mma16816(o[nt][k], r[0], r[1], r[2], r[3], ph[nt][0], ph[nt][1]);
-          mma16816(o[nt][k], r[0], r[1], r[2], r[3], pl[nt][0], pl[nt][1]);
+        for (int k = 0; k < kBlocks; ++k) {
+          uint32_t r[4];
+          ldsm4t(r, at + k * 32);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma16816(o[nt][k], r[0], r[1], r[2], r[3], ph[nt][u][0], ph[nt][u][1]);
+            mma16816(o[nt][k], r[0], r[1], r[2], r[3], pl[nt][u][0], pl[nt][u][1]);
+          }
         }
-      }
-    } else {
-      const uint32_t at = vt + ((lane & 7) + (lane & 8)) * S::kPitch;
+      } else {
+        const uint32_t at = vt + ((lane & 7) + (lane & 8)) * S::kPitch + (lane >> 4) * 16;
 #pragma unroll
-      for (int k = 0; k < kBlocks; k += 2) {
-        uint32_t r[4];
-        if (k + 1 < kBlocks) ldsm4t(r, at + k * 16 + (lane >> 4) * 16);
-        else ldsm2t(r[0], r[1], at + k * 16);
+        for (int k = 0; k < kBlocks; k += 2) {
+          uint32_t r[4];
+          if (k + 1 < kBlocks) ldsm4t(r, at + k * 16);
+          else ldsm2t(r[0], r[1], at + k * 16);
 #pragma unroll
-        for (int u = 0; u < 2 && k + u < kBlocks; ++u) {
-          // bytes: token 2c dims 2g, 2g + 1, token 2c + 1 the same; paired by dim
-          const uint32_t lo = __byte_perm(r[2 * u], 0, 0x3120);
-          const uint32_t hi = __byte_perm(r[2 * u + 1], 0, 0x3120);
-          const uint32_t a0 = widen(lo), a1 = widen(lo >> 16), a2 = widen(hi), a3 = widen(hi >> 16);
+          for (int x = 0; x < 2 && k + x < kBlocks; ++x) {
+            // bytes: token 2c dims 2g, 2g + 1, token 2c + 1 the same; paired by dim
+            const uint32_t lo = __byte_perm(r[2 * x], 0, 0x3120);
+            const uint32_t hi = __byte_perm(r[2 * x + 1], 0, 0x3120);
+            const uint32_t a0 = widen(lo), a1 = widen(lo >> 16);
+            const uint32_t a2 = widen(hi), a3 = widen(hi >> 16);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-            mma_f16(o[nt][k + u], a0, a1, a2, a3, ph[nt][0], ph[nt][1]);
+            for (int nt = 0; nt < NT; ++nt)
+              mma_f16(o[nt][k + x], a0, a1, a2, a3, ph[nt][u][0], ph[nt][u][1]);
+          }
         }
       }
     }
@@ -566,6 +642,11 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
   if (count > 0) {
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) load(i);
+    // the first segment's q comes while the first tiles do
+    open = true;
+    from_start = s_begin[warp].z == 0;
+    begin_segment(s_begin[warp].x, s_begin[warp].y);
+    seg_end = begin + tiles_of(s_begin[warp].w) - s_begin[warp].z;
     int stage = 0, free_stage = kStages - 1;
     for (int i = 0; i < count; ++i) {
       cp_wait<kStages - 2>();
@@ -573,8 +654,7 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
       load(free_stage);
       const int4 info = s_info[warp][stage];
       if (!open) {
-        open = true;
-        from_start = i > 0 || s_begin[warp].z == 0;
+        open = from_start = true;
         begin_segment(info.x, info.y);
         seg_end = begin + i + info.w;
       }
@@ -610,9 +690,9 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
   if (lane == 0) {
     s_tail[warp] = make_int4(tail, sb, shc, 0);
     Split sp{-1, 0, 0, 0};
-    if ((tail & 3) == 3) {  // its last tile's worker: the largest w with w * total / workers <= it
-      const int64_t last = (seg_end * workers + total - 1) / total - 1;
-      sp = Split{sb, shc, static_cast<int32_t>(last), (last + 1) * total / workers > seg_end};
+    if ((tail & 3) == 3) {
+      const int last = line.worker_of(seg_end - 1);
+      sp = Split{sb, shc, last, line.begin(last + 1) > seg_end};
     }
     s_split[warp] = sp;
   }
@@ -629,25 +709,33 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
     float* const slot = a.ws + slot_of(first_worker + w0, 0) * S::kSlot;
     for (int at = warp; at < NT * kBlocks; at += kWarps) {
       const int nt = at / kBlocks, k = at % kBlocks;
+      float2 ms[kWarps], ls[kWarps];
+      float4 vs[kWarps];
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {  // warps outside the run weigh nothing
+        const float* p = reinterpret_cast<const float*>(
+            ring_mem + static_cast<size_t>(min(max(w, w0), w1)) * kStages * S::kTileBytes);
+        ms[w] = *reinterpret_cast<const float2*>(p + S::kOut + nt * 8 + 2 * c);
+        ls[w] = *reinterpret_cast<const float2*>(p + S::kOut + NT * 8 + nt * 8 + 2 * c);
+        vs[w] = reinterpret_cast<const float4*>(p)[at * 32 + lane];
+      }
       float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      auto part = [&](int w) {
-        return reinterpret_cast<const float*>(ring_mem + static_cast<size_t>(w) * kStages * S::kTileBytes);
-      };
-      for (int w = w0; w <= w1; ++w)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) top[j] = fmaxf(top[j], part(w)[S::kOut + nt * 8 + 2 * c + j]);
-      for (int w = w0; w <= w1; ++w) {
-        const float* p = part(w);
-        const float x0 = weight_of(p[S::kOut + nt * 8 + 2 * c], top[0]);
-        const float x1 = weight_of(p[S::kOut + nt * 8 + 2 * c + 1], top[1]);
-        const float4 v = reinterpret_cast<const float4*>(p)[at * 32 + lane];
-        sum[0] += x0 * p[S::kOut + NT * 8 + nt * 8 + 2 * c];
-        sum[1] += x1 * p[S::kOut + NT * 8 + nt * 8 + 2 * c + 1];
-        acc.x += x0 * v.x;
-        acc.y += x1 * v.y;
-        acc.z += x0 * v.z;
-        acc.w += x1 * v.w;
+      for (int w = 0; w < kWarps; ++w) {
+        top[0] = fmaxf(top[0], ms[w].x);
+        top[1] = fmaxf(top[1], ms[w].y);
+      }
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        if (w < w0 || w > w1) continue;
+        const float x0 = weight_of(ms[w].x, top[0]), x1 = weight_of(ms[w].y, top[1]);
+        sum[0] += x0 * ls[w].x;
+        sum[1] += x1 * ls[w].y;
+        acc.x += x0 * vs[w].x;
+        acc.y += x1 * vs[w].y;
+        acc.z += x0 * vs[w].z;
+        acc.w += x1 * vs[w].w;
       }
       if (whole) {
         R::store(a, head.y, head.z, nt, k, acc, R::inverse(a, head.z, sum[0]),
@@ -671,57 +759,121 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
   if (threadIdx.x < kWarps) splits[first_worker + threadIdx.x] = s_split[threadIdx.x];
 }
 
-// Joins the partial results of the segments that cross CTAs: one CTA for each worker at
-// which such a segment begins.
+// Running sum of partial results: (top, sum, acc) of two heads per lane.
+struct Joined {
+  float top0 = -INFINITY, top1 = -INFINITY, sum0 = 0.f, sum1 = 0.f;
+  float4 acc = {0.f, 0.f, 0.f, 0.f};
+  __device__ __forceinline__ void add(float m0, float m1, float l0, float l1, const float4& v) {
+    const float t0 = fmaxf(top0, m0), t1 = fmaxf(top1, m1);
+    const float a0 = weight_of(top0, t0), a1 = weight_of(top1, t1);
+    const float b0 = weight_of(m0, t0), b1 = weight_of(m1, t1);
+    sum0 = sum0 * a0 + l0 * b0;
+    sum1 = sum1 * a1 + l1 * b1;
+    acc.x = acc.x * a0 + v.x * b0;
+    acc.y = acc.y * a1 + v.y * b1;
+    acc.z = acc.z * a0 + v.z * b0;
+    acc.w = acc.w * a1 + v.w * b1;
+    top0 = t0;
+    top1 = t1;
+  }
+};
+
+// Joins the partial results of the segments that cross warps' runs. CTA (x, y) takes the
+// splits that CTA x of the main kernel left, output blocks y, y + gridDim.y, ... Most
+// splits are between two neighbours in one CTA: two parts, one warp each split. At most
+// one goes on into further CTAs (up to every SM for one long request): its parts are
+// dealt to the four warps, each loading eight at a time, and joined in shared memory, so
+// the joining of a request split over 19 CTAs waits for memory twice, not 19 times.
+constexpr int kJoinWarps = 4, kJoinBatch = 8, kJoinY = 8;
+
 template <int D, bool kE4m3, int NT>
-__global__ void __launch_bounds__(128) paged_join_kernel(PagedArgs a) {
+__global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(PagedArgs a) {
   using S = Shape<D, kE4m3, NT>;
   using R = Rows<D, kE4m3, NT>;
   constexpr int kWarps = S::kWarps;
+  __shared__ float4 s_acc[kJoinWarps][32];
+  __shared__ float4 s_ml[kJoinWarps][32];
   allow_dependent_launch();
   wait_prerequisite();
-  const int64_t w0 = blockIdx.x;
-  const Split sp = reinterpret_cast<const Split*>(a.ws + slot_of(gridDim.x, 0) * S::kSlot)[w0];
-  if (sp.b < 0) return;
-  const int lane = threadIdx.x & 31, c = lane & 3;
-  // parts in line order: the tail slot of w0, the tail slots of the first workers of the
-  // CTAs behind it, the head slot of the last worker if its run goes on
-  const int64_t last_tail = sp.last - sp.head;
-  const int mid = static_cast<int>(last_tail / kWarps - w0 / kWarps);  // >= 0: last_tail >= w0
-  const int parts = 1 + mid + sp.head;
-  auto part = [&](int i) -> const float* {
-    const int64_t s = i == 0 ? slot_of(w0, 0)
-                      : i <= mid ? slot_of((w0 / kWarps + i) * kWarps, 0)
-                                 : slot_of(sp.last, 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane & 3;
+  const Split* splits = reinterpret_cast<const Split*>(
+      a.ws + slot_of(static_cast<int64_t>(gridDim.x) * kWarps, 0) * S::kSlot);
+  const int first_worker = blockIdx.x * kWarps;
+  int4 mine = make_int4(-1, 0, 0, 0);
+  if (lane < kWarps) mine = reinterpret_cast<const int4*>(splits)[first_worker + lane];
+  // a segment that ends in the CTA it begins in has its tail slot and one head slot
+  const int mid_mine = (mine.z - mine.w) / kWarps - static_cast<int>(blockIdx.x);
+  const unsigned near = __ballot_sync(0xffffffffu, mine.x >= 0 && mid_mine == 0);
+  const unsigned far = __ballot_sync(0xffffffffu, mine.x >= 0 && mid_mine > 0);
+
+  auto add = [&](Joined& j, const float* p, int nt, int at) {
+    const float2 m = *reinterpret_cast<const float2*>(p + S::kOut + nt * 8 + 2 * c);
+    const float2 l = *reinterpret_cast<const float2*>(p + S::kOut + NT * 8 + nt * 8 + 2 * c);
+    j.add(m.x, m.y, l.x, l.y, reinterpret_cast<const float4*>(p)[at * 32 + lane]);
+  };
+  auto finish = [&](const Joined& j, int b, int hc, int nt, int k) {
+    R::store(a, b, hc, nt, k, j.acc, R::inverse(a, hc, j.sum0), R::inverse(a, hc, j.sum1), lane);
+    if (k == 0) R::store_lse(a, b, hc, nt, j.top0, j.sum0, j.top1, j.sum1, lane);
+  };
+
+  unsigned left = near;
+  for (int turn = 0; left; ++turn, left &= left - 1) {
+    const int i = __ffs(left) - 1;
+    const int b = __shfl_sync(0xffffffffu, mine.x, i), hc = __shfl_sync(0xffffffffu, mine.y, i);
+    const int last = __shfl_sync(0xffffffffu, mine.z, i);
+    if (turn % kJoinWarps != warp) continue;
+    for (int at = blockIdx.y; at < NT * S::kBlocks; at += gridDim.y) {
+      const int nt = at / S::kBlocks;
+      Joined j;
+      add(j, a.ws + slot_of(first_worker + i, 0) * S::kSlot, nt, at);
+      add(j, a.ws + slot_of(last, 1) * S::kSlot, nt, at);
+      finish(j, b, hc, nt, at % S::kBlocks);
+    }
+  }
+  if (!far) return;
+  const int i = __ffs(far) - 1;
+  const int b = __shfl_sync(0xffffffffu, mine.x, i), hc = __shfl_sync(0xffffffffu, mine.y, i);
+  const int last = __shfl_sync(0xffffffffu, mine.z, i), head = __shfl_sync(0xffffffffu, mine.w, i);
+  const int mid = __shfl_sync(0xffffffffu, mid_mine, i);
+  // parts in line order: the tail slot of the first worker, the tail slots of the first
+  // workers of the CTAs behind it, the head slot of the last worker if its run goes on
+  const int parts = 1 + mid + head;
+  auto part = [&](int x) -> const float* {
+    const int64_t s = x == 0     ? slot_of(first_worker + i, 0)
+                      : x <= mid ? slot_of(static_cast<int64_t>(blockIdx.x + x) * kWarps, 0)
+                                 : slot_of(last, 1);
     return a.ws + s * S::kSlot;
   };
-  for (int at = threadIdx.x >> 5; at < NT * S::kBlocks; at += 4) {
-    const int nt = at / S::kBlocks, k = at % S::kBlocks;
-    float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int i = 0; i < parts; ++i) {
-      const float2 x = *reinterpret_cast<const float2*>(part(i) + S::kOut + nt * 8 + 2 * c);
-      top[0] = fmaxf(top[0], x.x);
-      top[1] = fmaxf(top[1], x.y);
+  for (int at = blockIdx.y; at < NT * S::kBlocks; at += gridDim.y) {
+    const int nt = at / S::kBlocks;
+    Joined j;
+    for (int x0 = warp; x0 < parts; x0 += kJoinWarps * kJoinBatch) {
+      float2 m[kJoinBatch], l[kJoinBatch];
+      float4 v[kJoinBatch];
+#pragma unroll
+      for (int u = 0; u < kJoinBatch; ++u) {  // all loads first; absent parts weigh nothing
+        const int x = x0 + u * kJoinWarps;
+        const float* p = part(min(x, parts - 1));
+        m[u] = *reinterpret_cast<const float2*>(p + S::kOut + nt * 8 + 2 * c);
+        l[u] = *reinterpret_cast<const float2*>(p + S::kOut + NT * 8 + nt * 8 + 2 * c);
+        v[u] = reinterpret_cast<const float4*>(p)[at * 32 + lane];
+      }
+#pragma unroll
+      for (int u = 0; u < kJoinBatch; ++u)
+        if (x0 + u * kJoinWarps < parts) j.add(m[u].x, m[u].y, l[u].x, l[u].y, v[u]);
     }
-#pragma unroll 4
-    for (int i = 0; i < parts; ++i) {
-      const float* p = part(i);
-      const float2 x = *reinterpret_cast<const float2*>(p + S::kOut + nt * 8 + 2 * c);
-      const float2 y = *reinterpret_cast<const float2*>(p + S::kOut + NT * 8 + nt * 8 + 2 * c);
-      const float4 v = reinterpret_cast<const float4*>(p)[at * 32 + lane];
-      const float x0 = weight_of(x.x, top[0]), x1 = weight_of(x.y, top[1]);
-      sum[0] += x0 * y.x;
-      sum[1] += x1 * y.y;
-      acc.x += x0 * v.x;
-      acc.y += x1 * v.y;
-      acc.z += x0 * v.z;
-      acc.w += x1 * v.w;
+    s_acc[warp][lane] = j.acc;
+    s_ml[warp][lane] = make_float4(j.top0, j.top1, j.sum0, j.sum1);
+    __syncthreads();
+    if (warp == 0) {
+      Joined all;
+#pragma unroll
+      for (int w = 0; w < kJoinWarps; ++w)
+        all.add(s_ml[w][lane].x, s_ml[w][lane].y, s_ml[w][lane].z, s_ml[w][lane].w,
+                s_acc[w][lane]);
+      finish(all, b, hc, nt, at % S::kBlocks);
     }
-    R::store(a, sp.b, sp.hc, nt, k, acc, R::inverse(a, sp.hc, sum[0]),
-             R::inverse(a, sp.hc, sum[1]), lane);
-    if (k == 0) R::store_lse(a, sp.b, sp.hc, nt, top[0], sum[0], top[1], sum[1], lane);
+    __syncthreads();
   }
 }
 
@@ -729,7 +881,8 @@ __global__ void __launch_bounds__(128) paged_join_kernel(PagedArgs a) {
 template <int D, bool kE4m3, int NT>
 int64_t grid_of(const PagedArgs& a) {
   using S = Shape<D, kE4m3, NT>;
-  const int64_t tiles = (a.max_len + kTile - 1) / kTile * a.batch * a.hkv * a.chunks;
+  const int64_t tiles =
+      (static_cast<int64_t>(a.max_len) + S::kTile - 1) / S::kTile * a.batch * a.hkv * a.chunks;
   int64_t ctas = std::min<int64_t>(sm_count(), kMaxWorkers / S::kWarps);
   return std::max<int64_t>(1, std::min(ctas, (tiles + S::kWarps - 1) / S::kWarps));
 }
@@ -750,7 +903,8 @@ void launch(PagedArgs a, cudaStream_t st) {
   });
   const unsigned ctas = static_cast<unsigned>(grid_of<D, kE4m3, NT>(a));
   launch_pdl(paged_attn_kernel<D, kE4m3, NT>, dim3(ctas), dim3(S::kWarps * 32), S::kSmem, st, a);
-  launch_pdl(paged_join_kernel<D, kE4m3, NT>, dim3(ctas * S::kWarps), dim3(128), 0, st, a);
+  launch_pdl(paged_join_kernel<D, kE4m3, NT>, dim3(ctas, std::min(kJoinY, NT * S::kBlocks)),
+             dim3(kJoinWarps * 32), 0, st, a);
 }
 
 // Up to 8 query heads per KV head use one column tile; wider groups two, which halves the
@@ -812,6 +966,11 @@ extern "C" int umic_paged_attention(
                 "%s: num_pages * page_size, max_pages * page_size and batch * hq must stay below "
                 "2^31",
                 me);
+  // tiles of every segment, had every request the longest row, count in 32 bits
+  const int64_t segments = static_cast<int64_t>(batch) * hkv * ((hq / hkv + 7) / 8);
+  if (segments > 0x7fffffffLL / std::max<int64_t>(1, max_pages * page_size / kSub))
+    return fail(UMIC_ERR_UNSUPPORTED,
+                "%s: batch * KV heads * max_pages * page_size / 16 must stay below 2^31", me);
   if (batch == 0) return UMIC_OK;
   if (!q || !k_pages || !v_pages || !kv_lens || !out || (max_pages > 0 && !block_table))
     return fail(UMIC_ERR_INVALID_ARG, "%s: null pointer", me);
@@ -842,7 +1001,7 @@ extern "C" int umic_paged_attention(
   a.q_sb = q_sb; a.q_sh = q_sh; a.o_sb = o_sb; a.o_sh = o_sh;
   a.pg_sp = pg_sp * es; a.pg_sh = pg_sh * es; a.pg_ss = pg_ss * es;
   a.table_stride = table_stride;
-  a.max_len = max_pages * page_size;
+  a.max_len = static_cast<int32_t>(max_pages * page_size);
   a.num_pages = num_pages;
   a.page_size = static_cast<int32_t>(page_size);
   a.hq = hq; a.hkv = hkv; a.batch = static_cast<int32_t>(batch); a.group = hq / hkv;
