@@ -291,10 +291,11 @@ UMIC_API int umic_paged_attention(
     int64_t o_sh, float* lse, int64_t batch, int32_t hq, int32_t hkv, int32_t head_dim,
     float scale, void* workspace, size_t workspace_bytes, void* stream);
 
-/* Bytes of workspace umic_paged_attention needs for these heads on the current device,
- * whatever the batch and lengths. */
-UMIC_API size_t umic_paged_attention_workspace_bytes(int32_t hq, int32_t hkv,
-                                                     int32_t head_dim);
+/* Bytes of workspace umic_paged_attention needs for these sizes on the current device,
+ * whatever the lengths. */
+UMIC_API size_t umic_paged_attention_workspace_bytes(int64_t batch, int32_t hq, int32_t hkv,
+                                                     int32_t head_dim, int64_t max_pages,
+                                                     int64_t page_size, int cache_dtype);
 
 /* ---- attention over a cached prefix -------------------------------------- */
 

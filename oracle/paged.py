@@ -84,29 +84,32 @@ def norm_mrope(x, weight, eps, positions, inv_freq, sections, interleaved, scali
     return y, torch.cat((mag, mag, rest.abs()), -1)
 
 
-def paged_attention(q, k_pages, v_pages, table, lens, scale, k_scale=None, v_scale=None):
-    """(out, lse, spread, reach) in fp64; a row's tokens on pages outside the pool are left
-    out. For error bounds: spread = sum_j p_j |v_j|, and reach = max_j scale * sum |q| |k_j|."""
-    q = q.detach().cpu().double()
+def paged_attention(q, k_pages, v_pages, table, lens, scale, k_scale=None, v_scale=None,
+                    device="cpu"):
+    """(out, lse, spread, reach) in fp64 CPU tensors, computed on `device`; a row's tokens on
+    pages outside the pool are left out. For error bounds: spread = sum_j p_j |v_j|, and
+    reach = max_j scale * sum |q| |k_j|."""
+    q = q.detach().to(device).double()
     b, hq, d = q.shape
     num, hk, page, _ = k_pages.shape
 
-    def values(pages, s):
-        x = pages.detach().cpu()
-        x = (x.float() if x.element_size() == 1 else x).double()
-        return x if s is None else x * s.detach().cpu().double().view(1, -1, 1, 1)
+    def values(pages, s, ids, at):
+        x = pages.detach().to(device)
+        x = x.view(torch.uint8)[ids, :, at].view(x.dtype) if x.element_size() == 1 else x[ids, :, at]
+        x = (x.float() if x.element_size() == 1 else x).double().transpose(0, 1)
+        return x if s is None else x * s.detach().to(device).double().view(-1, 1, 1)
 
-    kp, vp = values(k_pages, k_scale), values(v_pages, v_scale)
     out, spread = torch.zeros(b, hq, d).double(), torch.zeros(b, hq, d).double()
     lse, reach = torch.full((b, hq), float("-inf")).double(), torch.zeros(b, hq).double()
     for r in range(b):
         n = min(max(int(lens[r]), 0), table.shape[1] * page)
-        at = [(int(table[r, j // page]), j % page) for j in range(n)]
-        at = [(p, o) for p, o in at if 0 <= p < num]
-        if not at:
+        j = torch.arange(n)
+        ids, at = table[r].cpu().long()[j // page], j % page
+        there = (ids >= 0) & (ids < num)
+        if not bool(there.any()):
             continue
-        p_i, o_i = (torch.tensor(x) for x in zip(*at))
-        k, v = kp[p_i, :, o_i].transpose(0, 1), vp[p_i, :, o_i].transpose(0, 1)
+        ids, at = ids[there].to(device), at[there].to(device)
+        k, v = values(k_pages, k_scale, ids, at), values(v_pages, v_scale, ids, at)
         qr = q[r].view(hk, hq // hk, d)
         s = qr @ k.transpose(1, 2) * scale
         lse[r] = torch.logsumexp(s, -1).reshape(hq)

@@ -296,8 +296,9 @@ def _attend_case(seed, lens, hq, hk, d, page, e4m3, dev, order="phsd", spare=2, 
     return q, kp, vp, table, lens, d ** -0.5, ks, vs
 
 
-def _check_attend(cuda, q, kp, vp, table, lens, scale, ks, vs, **kw):
-    want, lse, spread, reach = oracle.paged_attention(q, kp, vp, table, lens, scale, ks, vs)
+def _check_attend(cuda, q, kp, vp, table, lens, scale, ks, vs, device="cpu", **kw):
+    want, lse, spread, reach = oracle.paged_attention(q, kp, vp, table, lens, scale, ks, vs,
+                                                      device)
     out, got_lse = paged_attention(q, kp, vp, table.to(cuda), lens.to(cuda), scale, k_scale=ks,
                                    v_scale=vs, return_lse=True, **kw)
     d, longest = q.shape[2], int(lens.max())
@@ -346,6 +347,33 @@ def test_attend_long_and_many(cuda, batch, longest, e4m3):
     lens[batch // 2] = longest
     c = _attend_case(batch, lens, 8, 2, 128, 16, e4m3, cuda)
     _check_attend(cuda, *c)
+
+
+@pytest.mark.parametrize("heads", HEADS[:7], ids=lambda h: "x".join(map(str, h)))
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("lens", [[0, 0, 0], [1, 0, 0], [40, 700, 0], [2000, 3, 1100]])
+def test_attend_wide_table(cuda, heads, e4m3, lens):
+    """A table whose rows could hold far more than the requests do."""
+    c = _attend_case(7, lens, *heads, 64, e4m3, cuda, width=40000)
+    _check_attend(cuda, *c)
+
+
+@pytest.mark.parametrize("heads,e4m3,batch,longest", [
+    ((32, 8, 128), False, 40, 4500), ((16, 8, 128), True, 300, 2000), ((16, 1, 64), False, 3, 900000),
+    ((24, 3, 256), True, 5, 52000), ((16, 16, 80), False, 1, 90000)])
+def test_attend_large(cuda, heads, e4m3, batch, longest):
+    """Enough tiles that the warps claim their work; the same bits every time."""
+    g = _gen(batch)
+    lens = (torch.rand(batch, generator=g) * longest).long()
+    lens[batch // 2], lens[-1] = longest, longest - 5
+    lens[3::17] = 0
+    c = _attend_case(batch, lens.tolist(), *heads, 64, e4m3, cuda)
+    out, lse = _check_attend(cuda, *c, device=cuda)
+    q, kp, vp, table, lens, scale, ks, vs = c
+    for _ in range(3):
+        again = paged_attention(q, kp, vp, table.to(cuda), lens.to(cuda), scale, k_scale=ks,
+                                v_scale=vs, return_lse=True)
+        assert torch.equal(again[0], out) and torch.equal(again[1], lse)
 
 
 def test_attend_every_length_of_a_tile(cuda):

@@ -44,6 +44,34 @@ constexpr float kF16Shift = 14.f;     // e4m3 path: weights are held as 2^14 p
 constexpr int kSmemBudget = 216 * 1024;
 constexpr int64_t kMaxWorkers = 2048;  // warps of the main kernel, bounds the workspace
 
+// A split segment, left by the run that holds its first tile for the joining kernel.
+struct Split {
+  int32_t b;     // request, or -1: none begins here
+  int32_t hc;    // segment of the request
+  int32_t last;  // run that holds its last tile
+  int32_t head;  // 1: that run goes on behind the segment
+};
+
+// The workspace: a header, where each run begins, the splits, and two partial results for
+// each run (0: of its last segment, 1: of its first if that is another).
+struct Header {
+  int32_t total, big, runs, next;  // tiles of the line and of its big runs; runs; runs claimed
+  int32_t pad[12];
+};
+struct Space {
+  char* base;
+  int64_t runs;  // room for
+  __host__ __device__ Header* header() const { return reinterpret_cast<Header*>(base); }
+  __host__ __device__ int4* starts() const { return reinterpret_cast<int4*>(base + sizeof(Header)); }
+  __host__ __device__ Split* splits() const { return reinterpret_cast<Split*>(starts() + runs); }
+  __host__ __device__ float* slot(int64_t run, int head, int floats) const {
+    return reinterpret_cast<float*>(splits() + runs) + (run * 2 + head) * floats;
+  }
+  static constexpr size_t bytes(int64_t runs, int64_t floats) {
+    return sizeof(Header) + runs * (sizeof(int4) + sizeof(Split) + 2 * floats * sizeof(float));
+  }
+};
+
 struct PagedArgs {
   const __nv_bfloat16* q;
   const char *k_pages, *v_pages;
@@ -52,7 +80,7 @@ struct PagedArgs {
   __nv_bfloat16* out;
   float* lse;
   uint32_t* err;
-  float* ws;
+  Space ws;
   int64_t q_sb, q_sh, pg_sp, pg_sh, pg_ss;  // pg_* in bytes
   int64_t table_stride, num_pages, o_sb, o_sh;
   int32_t max_len, page_size, hq, hkv, batch, group, chunks;  // chunks: segments per KV head
@@ -81,16 +109,6 @@ struct Shape {
   static_assert(kStages >= 2, "one tile in use, one in flight");
   static_assert(kStages * kTileBytes >= kSlot * 4, "a partial result fits its warp's ring");
 };
-
-// A split segment, left by the warp that holds its first tile for the joining kernel.
-struct Split {
-  int32_t b;     // request, or -1: none begins here
-  int32_t hc;    // segment of the request
-  int32_t last;  // worker that holds its last tile
-  int32_t head;  // 1: that worker's run goes on behind the segment
-};
-
-__host__ __device__ constexpr int64_t slot_of(int64_t worker, int head) { return worker * 2 + head; }
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
@@ -172,9 +190,32 @@ struct Line {
   int base, longer;
   __device__ Line(int total, int workers) : base(total / workers), longer(total % workers) {}
   __device__ int begin(int w) const { return w * base + min(w, longer); }
-  __device__ int worker_of(int x) const {
+  __device__ int run_of(int x) const {
     const int cut = longer * (base + 1);
     return x < cut ? x / (base + 1) : longer + (x - cut) / base;
+  }
+};
+
+// Which runs a line is cut into when they are claimed as warps come free. At full HBM load
+// the SMs do not get equal shares (measured per SM on a 2 GB line: 470 to 650 thousand
+// cycles for equal runs, by their place on the chip), so each warp first has a run of
+// 11 / 16 of its equal share and the rest is cut into kSmall runs per warp: the warps that
+// are ahead take more of them. Which runs there are depends on the lengths alone, so sums
+// are taken alike whoever computes them.
+constexpr int kSmall = 4;
+constexpr int kLeastClaimed = 32;  // tiles a warp from which on the line is cut so
+template <bool kClaim>
+struct Cut {
+  Line big, small;
+  int big_tiles, workers;
+  __device__ Cut(int total, int big_total, int n)
+      : big(big_total, n), small(kClaim ? total - big_total : 0, kClaim ? n * kSmall : 1),
+        big_tiles(big_total), workers(n) {}
+  __device__ int begin(int r) const {
+    return !kClaim || r <= workers ? big.begin(r) : big_tiles + small.begin(r - workers);
+  }
+  __device__ int run_of(int x) const {
+    return !kClaim || x < big_tiles ? big.run_of(x) : workers + small.run_of(x - big_tiles);
   }
 };
 
@@ -231,7 +272,91 @@ __device__ __forceinline__ float weight_of(float m, float top) {
   return m == -INFINITY ? 0.f : exp2_fast(m - top);
 }
 
-template <int D, bool kE4m3, int NT>
+// Sums of the threads before this one, and of the block; two barriers' worth of one.
+template <int kWarps>
+__device__ __forceinline__ int block_sums(int mine, int* s_warp_sum, int* total) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += x;
+  }
+  if (lane == 31) s_warp_sum[warp] = upto;
+  __syncthreads();
+  int all = 0;
+  upto -= mine;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w == warp) upto += all;
+    all += s_warp_sum[w];
+  }
+  *total = all;
+  return upto;
+}
+
+// Zero rows of the requests without tokens, dealt to the CTAs.
+__device__ __forceinline__ void zero_empty(const PagedArgs& a, int d) {
+  for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
+    if (clamped_len(a, b) > 0) continue;
+    for (int i = threadIdx.x; i < a.hq * (d / 8); i += blockDim.x)
+      st_vec(a.out + b * a.o_sb + i / (d / 8) * a.o_sh + i % (d / 8) * 8, make_uint4(0, 0, 0, 0));
+    if (a.lse)
+      for (int h = threadIdx.x; h < a.hq; h += blockDim.x)
+        a.lse[static_cast<int64_t>(b) * a.hq + h] = -INFINITY;
+  }
+}
+
+// Cuts the line for claimed runs: the header and where each run begins. Every CTA scans
+// the lengths and places its share of the runs.
+constexpr int kCutThreads = 512, kCutCtas = 8, kCutBatch = 8192;
+__global__ void __launch_bounds__(kCutThreads) paged_cut_kernel(PagedArgs a, int d, int tile,
+                                                                int workers) {
+  extern __shared__ int s_first[];  // tile of the line at which each request begins
+  __shared__ int s_warp_sum[kCutThreads / 32];
+  allow_dependent_launch();
+  wait_prerequisite();
+  const int hcs = a.hkv * a.chunks;
+  const int per = (a.batch + kCutThreads - 1) / kCutThreads;
+  const int b0 = min(a.batch, static_cast<int>(threadIdx.x) * per), b1 = min(a.batch, b0 + per);
+  int mine = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int n = a.lens[b];
+    if (blockIdx.x == 0 && (n < 0 || n > a.max_len)) atomicOr(a.err, UMIC_DEVERR_BAD_PAGE);
+    s_first[b] = mine;
+    mine += (max(0, min(n, a.max_len)) + tile - 1) / tile;
+  }
+  int total;
+  const int upto = block_sums<kCutThreads / 32>(mine, s_warp_sum, &total);
+  for (int b = b0; b < b1; ++b) s_first[b] = (s_first[b] + upto) * hcs;
+  total *= hcs;
+  __syncthreads();
+  workers = min(workers, total);
+  const bool claimed = total >= workers * kLeastClaimed;
+  const int big = claimed ? total / 16 * 11 : total;
+  const int runs = claimed ? workers * (1 + kSmall) : workers;
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    Header* h = a.ws.header();
+    h->total = total;
+    h->big = big;
+    h->runs = runs;
+    h->next = workers;
+  }
+  const Cut<true> cut(total, big, max(workers, 1));
+  for (int r = blockIdx.x * kCutThreads + threadIdx.x; r < runs; r += gridDim.x * kCutThreads) {
+    const int at = cut.begin(r);
+    int lo = 0, hi = a.batch;  // the last request that begins at or before `at`: it has tiles
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (s_first[mid] <= at) lo = mid; else hi = mid;
+    }
+    const int len = clamped_len(a, lo), tiles = (len + tile - 1) / tile, in = at - s_first[lo];
+    a.ws.starts()[r] = make_int4(lo, in / tiles, in % tiles, len);
+  }
+  zero_empty(a, d);
+}
+
+template <int D, bool kE4m3, int NT, bool kClaim>
 __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
     paged_attn_kernel(PagedArgs a) {
   using S = Shape<D, kE4m3, NT>;
@@ -240,8 +365,11 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
   constexpr int kThreads = kWarps * 32, MT = S::MT, kTile = S::kTile;
   auto tiles_of = [](int len) { return (len + kTile - 1) / kTile; };
   extern __shared__ __align__(16) char ring_mem[];
-  __shared__ int4 s_info[kWarps][kStages];  // request, segment, valid rows (a byte per
-                                            // subtile), tiles left of the segment
+  // request (-1: no more tiles), segment, valid rows (a byte per subtile) and flags, tiles
+  // left of the segment
+  __shared__ int4 s_info[kWarps][kStages];
+  constexpr int kSegFirst = 1 << 16, kRunFirst = 1 << 17, kRunLast = 1 << 18;
+  __shared__ int s_run[kClaim ? kWarps : 1][kStages];
   __shared__ int4 s_begin[kWarps];          // request, segment, tile and request length at a
                                             // warp's start
   __shared__ int s_warp_sum[kWarps];
@@ -253,66 +381,49 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int hcs = a.hkv * a.chunks;  // segments per request
 
-  // ---- the line of tiles, and where each warp's run begins on it
-  const int per = (a.batch + kThreads - 1) / kThreads;
-  const int b0 = min(a.batch, static_cast<int>(threadIdx.x) * per), b1 = min(a.batch, b0 + per);
-  int mine = 0, first_len = 0;
-  for (int b = b0; b < b1; ++b) {
-    const int n = a.lens[b];
-    if (blockIdx.x == 0 && (n < 0 || n > a.max_len)) atomicOr(a.err, UMIC_DEVERR_BAD_PAGE);
-    const int len = max(0, min(n, a.max_len));
-    if (b == b0) first_len = len;
-    mine += tiles_of(len);
-  }
-  int upto = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += x;
-  }
-  if (lane == 31) s_warp_sum[warp] = upto;
-  __syncthreads();
-  int total = 0;
-  upto -= mine;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w == warp) upto += total;
-    total += s_warp_sum[w];
-  }
-  total *= hcs;
-  const int workers = min(static_cast<int>(gridDim.x) * kWarps, total);
   const int first_worker = static_cast<int>(blockIdx.x) * kWarps;
-  const Line line(total, max(workers, 1));
-  if (mine > 0 && first_worker < workers &&
-      line.begin(first_worker + kWarps) > upto * hcs) {
-    for (int w = 0; w < kWarps && first_worker + w < workers; ++w) {
-      int at = line.begin(first_worker + w) - upto * hcs;
-      if (at < 0 || at >= mine * hcs) continue;
-      int len = first_len;
-      for (int b = b0;; len = clamped_len(a, ++b)) {
-        const int tiles = tiles_of(len);
-        if (at < tiles * hcs) {
-          s_begin[w] = make_int4(b, at / tiles, at % tiles, len);
-          break;
+  int total, workers;
+  if constexpr (!kClaim) {
+    // ---- the line of tiles, and where each warp's run begins on it
+    const int per = (a.batch + kThreads - 1) / kThreads;
+    const int b0 = min(a.batch, static_cast<int>(threadIdx.x) * per), b1 = min(a.batch, b0 + per);
+    int mine = 0, first_len = 0;
+    for (int b = b0; b < b1; ++b) {
+      const int n = a.lens[b];
+      if (blockIdx.x == 0 && (n < 0 || n > a.max_len)) atomicOr(a.err, UMIC_DEVERR_BAD_PAGE);
+      const int len = max(0, min(n, a.max_len));
+      if (b == b0) first_len = len;
+      mine += tiles_of(len);
+    }
+    const int upto = block_sums<kWarps>(mine, s_warp_sum, &total);
+    total *= hcs;
+    workers = min(static_cast<int>(gridDim.x) * kWarps, total);
+    const Line line(total, max(workers, 1));
+    if (mine > 0 && first_worker < workers && line.begin(first_worker + kWarps) > upto * hcs) {
+      for (int w = 0; w < kWarps && first_worker + w < workers; ++w) {
+        int at = line.begin(first_worker + w) - upto * hcs;
+        if (at < 0 || at >= mine * hcs) continue;
+        int len = first_len;
+        for (int b = b0;; len = clamped_len(a, ++b)) {
+          const int tiles = tiles_of(len);
+          if (at < tiles * hcs) {
+            s_begin[w] = make_int4(b, at / tiles, at % tiles, len);
+            break;
+          }
+          at -= tiles * hcs;
         }
-        at -= tiles * hcs;
       }
     }
+    zero_empty(a, D);
+    __syncthreads();
+  } else {
+    total = a.ws.header()->total;
+    workers = min(static_cast<int>(gridDim.x) * kWarps, total);
   }
-  // requests without tokens: zeros
-  for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
-    if (clamped_len(a, b) > 0) continue;
-    for (int i = threadIdx.x; i < a.hq * (D / 8); i += kThreads)
-      st_vec(a.out + b * a.o_sb + i / (D / 8) * a.o_sh + i % (D / 8) * 8, make_uint4(0, 0, 0, 0));
-    if (a.lse)
-      for (int h = threadIdx.x; h < a.hq; h += kThreads)
-        a.lse[static_cast<int64_t>(b) * a.hq + h] = -INFINITY;
-  }
-  __syncthreads();
 
   const int worker = first_worker + warp;
-  const int begin = line.begin(worker);
-  const int count = worker < workers ? line.begin(worker + 1) - begin : 0;
+  const int runs = kClaim ? a.ws.header()->runs : workers;
+  const Cut<kClaim> cut(total, kClaim ? a.ws.header()->big : total, max(workers, 1));
   char* const ring = ring_mem + static_cast<size_t>(warp) * kStages * S::kTileBytes;
   const uint32_t ring_addr = smem_addr(ring);
 
@@ -331,26 +442,38 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
       }
     }
   };
-  if (count > 0) {
-    const int4 st = s_begin[warp];
+  // the run being copied, its tiles still to copy, and the run after it
+  int lrun = worker, left = 0, fresh = 0, next_run = 0;
+  int4 next_start;
+  auto start_run = [&](const int4& st) {
+    left = cut.begin(lrun + 1) - cut.begin(lrun);
+    fresh = kRunFirst;
     lb = st.x;
     lhc = st.y;
     lt = st.z;
     llen = st.w;
     ltiles = tiles_of(llen);
-    row_of_table += lb * a.table_stride;
+    row_of_table = a.table + lb * a.table_stride;
     lpi = lt * kTile / a.page_size;
     loff = lt * kTile - lpi * a.page_size;
     look_up();
+    if constexpr (kClaim) {  // the next one is claimed now and needed a run later
+      if (lane == 0) next_run = atomicAdd(&a.ws.header()->next, 1);
+      next_run = __shfl_sync(0xffffffffu, next_run, 0);
+      if (next_run < runs) next_start = a.ws.starts()[next_run];
+    }
+  };
+  int4 start = make_int4(0, 0, 0, 0);
+  if (worker < workers) {
+    start = kClaim ? a.ws.starts()[worker] : s_begin[warp];
+    start_run(start);
   }
   constexpr int kCols = S::kRow / 16;  // 16-byte pieces of a row
   constexpr int kCopies = (kSub * kCols + 31) / 32;
   const bool dense = a.pg_ss == S::kRow;  // a page's rows of a head lie one behind the other
   const int64_t v_minus_k = a.v_pages - a.k_pages;
-  int loaded = 0;
   auto load = [&](int stage) {
-    if (loaded < count) {
-      ++loaded;
+    if (left > 0) {
       int rows_of = 0;
       const int64_t head_at = lhc / a.chunks * a.pg_sh;
 #pragma unroll
@@ -390,8 +513,14 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
           }
         }
       }
-      if (lane == 0) s_info[warp][stage] = make_int4(lb, lhc, rows_of, ltiles - lt);
-      if (loaded < count) {
+      --left;
+      if (lane == 0) {
+        const int flags = fresh | (lt == 0 ? kSegFirst : 0) | (left == 0 ? kRunLast : 0);
+        s_info[warp][stage] = make_int4(lb, lhc, rows_of | flags, ltiles - lt);
+        if constexpr (kClaim) s_run[warp][stage] = lrun;
+      }
+      fresh = 0;
+      if (left > 0) {
         if (++lt == ltiles) {
           lt = lpi = loff = 0;
           if (++lhc == hcs) {
@@ -403,7 +532,12 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
           }
         }
         look_up();
+      } else if (kClaim && next_run < runs) {
+        lrun = next_run;
+        start_run(next_start);
       }
+    } else if (lane == 0) {
+      s_info[warp][stage].x = -1;
     }
     cp_commit();
   };
@@ -414,8 +548,6 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
   float o[NT][kBlocks][4];
   float m[NT][2], l[NT][2], fac[NT][2];
   int sb = 0, shc = 0;
-  bool open = false, from_start = false;
-  int seg_end = 0;  // line position behind the segment
 
   auto begin_segment = [&](int b, int hc) {
     sb = b;
@@ -637,35 +769,47 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
     }
   };
 
-  // ---- the run
+  auto split_of = [&](int seg_end) {
+    const int last = cut.run_of(seg_end - 1);
+    return Split{sb, shc, last, cut.begin(last + 1) > seg_end};
+  };
+
+  // ---- the run, or runs
   int tail = 0;  // 1: a partial segment is left in registers, 2: it has the first tile, 4: the last
-  if (count > 0) {
+  int pos = 0;   // line position
+  Split split{-1, 0, 0, 0};
+  if (worker < workers) {
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) load(i);
     // the first segment's q comes while the first tiles do
-    open = true;
-    from_start = s_begin[warp].z == 0;
-    begin_segment(s_begin[warp].x, s_begin[warp].y);
-    seg_end = begin + tiles_of(s_begin[warp].w) - s_begin[warp].z;
-    int stage = 0, free_stage = kStages - 1;
-    for (int i = 0; i < count; ++i) {
+    bool open = true, from_start = start.z == 0;
+    begin_segment(start.x, start.y);
+    int stage = 0, free_stage = kStages - 1, run = worker;
+    while (true) {
       cp_wait<kStages - 2>();
       __syncwarp();
       load(free_stage);
       const int4 info = s_info[warp][stage];
-      if (!open) {
-        open = from_start = true;
-        begin_segment(info.x, info.y);
-        seg_end = begin + i + info.w;
+      if (info.x < 0) break;
+      if (info.z & kRunFirst) {
+        if constexpr (kClaim) run = s_run[warp][stage];
+        pos = cut.begin(run);
       }
-      if (info.z > 0) tile(stage, info.z);
+      if (!open) {
+        open = true;
+        from_start = info.z & kSegFirst;
+        begin_segment(info.x, info.y);
+      }
+      ++pos;
+      if (info.z & 0xffff) tile(stage, info.z);
       free_stage = stage;
       stage = stage + 1 == kStages ? 0 : stage + 1;
-      const bool done = info.w == 1;
-      if (done || i + 1 == count) {
+      const bool done = info.w == 1, run_ends = info.z & kRunLast;
+      if (done || run_ends) {
         sum_l();
         open = false;
-        if (done && from_start) {
+        const bool whole = done && from_start;
+        if (whole) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             const float i0 = R::inverse(a, shc, l[nt][0]), i1 = R::inverse(a, shc, l[nt][1]);
@@ -676,10 +820,17 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
                        lane);
             R::store_lse(a, sb, shc, nt, m[nt][0], l[nt][0], m[nt][1], l[nt][1], lane);
           }
-        } else if (i + 1 < count) {
-          store_slot(a.ws + slot_of(worker, 1) * S::kSlot);
+        } else if (kClaim || !run_ends) {
+          store_slot(a.ws.slot(run, run_ends ? 0 : 1, S::kSlot));
         } else {
           tail = 1 | (from_start ? 2 : 0) | (done ? 4 : 0);
+        }
+        if (run_ends) {
+          if (from_start && !done) split = split_of(pos + info.w - 1);
+          if constexpr (kClaim) {
+            if (lane == 0) a.ws.splits()[run] = split;
+            split.b = -1;
+          }
         }
       }
     }
@@ -687,14 +838,10 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
     __syncwarp();
     if (tail) store_slot(reinterpret_cast<float*>(ring));
   }
+  if constexpr (kClaim) return;
   if (lane == 0) {
     s_tail[warp] = make_int4(tail, sb, shc, 0);
-    Split sp{-1, 0, 0, 0};
-    if ((tail & 3) == 3) {
-      const int last = line.worker_of(seg_end - 1);
-      sp = Split{sb, shc, last, line.begin(last + 1) > seg_end};
-    }
-    s_split[warp] = sp;
+    s_split[warp] = split;
   }
   __syncthreads();
 
@@ -706,7 +853,7 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
     int w1 = w0;
     while (w1 + 1 < kWarps && (s_tail[w1 + 1].x & 3) == 1) ++w1;
     const bool whole = (head.x & 2) && (s_tail[w1].x & 4);
-    float* const slot = a.ws + slot_of(first_worker + w0, 0) * S::kSlot;
+    float* const slot = a.ws.slot(first_worker + w0, 0, S::kSlot);
     for (int at = warp; at < NT * kBlocks; at += kWarps) {
       const int nt = at / kBlocks, k = at % kBlocks;
       float2 ms[kWarps], ls[kWarps];
@@ -754,9 +901,7 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
     if (whole && threadIdx.x == 0) s_split[w0].b = -1;
   }
   __syncthreads();
-  Split* const splits =
-      reinterpret_cast<Split*>(a.ws + slot_of(static_cast<int64_t>(gridDim.x) * kWarps, 0) * S::kSlot);
-  if (threadIdx.x < kWarps) splits[first_worker + threadIdx.x] = s_split[threadIdx.x];
+  if (threadIdx.x < kWarps) a.ws.splits()[first_worker + threadIdx.x] = s_split[threadIdx.x];
 }
 
 // Running sum of partial results: (top, sum, acc) of two heads per lane.
@@ -778,15 +923,15 @@ struct Joined {
   }
 };
 
-// Joins the partial results of the segments that cross warps' runs. CTA (x, y) takes the
-// splits that CTA x of the main kernel left, output blocks y, y + gridDim.y, ... Most
-// splits are between two neighbours in one CTA: two parts, one warp each split. At most
-// one goes on into further CTAs (up to every SM for one long request): its parts are
-// dealt to the four warps, each loading eight at a time, and joined in shared memory, so
-// the joining of a request split over 19 CTAs waits for memory twice, not 19 times.
 constexpr int kJoinWarps = 4, kJoinBatch = 8, kJoinY = 8;
 
-template <int D, bool kE4m3, int NT>
+// Joins the partial results of the segments that cross runs. CTA (x, y) takes the splits
+// left by runs x * kWarps on (those of CTA x of the main kernel, where runs are not
+// claimed), output blocks y, y + gridDim.y, ... A split between two neighbours has two
+// parts: one warp each. A longer one (up to every run, for one long request) has its parts
+// dealt to the four warps, each loading eight at a time, and joined in shared memory: the
+// joining of 19 parts waits for memory twice, not 19 times.
+template <int D, bool kE4m3, int NT, bool kClaim>
 __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(PagedArgs a) {
   using S = Shape<D, kE4m3, NT>;
   using R = Rows<D, kE4m3, NT>;
@@ -796,15 +941,16 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(PagedArgs a
   allow_dependent_launch();
   wait_prerequisite();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane & 3;
-  const Split* splits = reinterpret_cast<const Split*>(
-      a.ws + slot_of(static_cast<int64_t>(gridDim.x) * kWarps, 0) * S::kSlot);
-  const int first_worker = blockIdx.x * kWarps;
+  const int first = blockIdx.x * kWarps;
   int4 mine = make_int4(-1, 0, 0, 0);
-  if (lane < kWarps) mine = reinterpret_cast<const int4*>(splits)[first_worker + lane];
-  // a segment that ends in the CTA it begins in has its tail slot and one head slot
-  const int mid_mine = (mine.z - mine.w) / kWarps - static_cast<int>(blockIdx.x);
+  if (lane < kWarps && (!kClaim || first + lane < a.ws.header()->runs))
+    mine = reinterpret_cast<const int4*>(a.ws.splits())[first + lane];
+  // parts between the first run's and the last one's: of every run, or (joined already in
+  // the CTA) of every further CTA
+  const int mid_mine = kClaim ? mine.z - mine.w - (first + lane)
+                              : (mine.z - mine.w) / kWarps - static_cast<int>(blockIdx.x);
   const unsigned near = __ballot_sync(0xffffffffu, mine.x >= 0 && mid_mine == 0);
-  const unsigned far = __ballot_sync(0xffffffffu, mine.x >= 0 && mid_mine > 0);
+  unsigned far = __ballot_sync(0xffffffffu, mine.x >= 0 && mid_mine > 0);
 
   auto add = [&](Joined& j, const float* p, int nt, int at) {
     const float2 m = *reinterpret_cast<const float2*>(p + S::kOut + nt * 8 + 2 * c);
@@ -825,95 +971,119 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(PagedArgs a
     for (int at = blockIdx.y; at < NT * S::kBlocks; at += gridDim.y) {
       const int nt = at / S::kBlocks;
       Joined j;
-      add(j, a.ws + slot_of(first_worker + i, 0) * S::kSlot, nt, at);
-      add(j, a.ws + slot_of(last, 1) * S::kSlot, nt, at);
+      add(j, a.ws.slot(first + i, 0, S::kSlot), nt, at);
+      add(j, a.ws.slot(last, 1, S::kSlot), nt, at);
       finish(j, b, hc, nt, at % S::kBlocks);
     }
   }
-  if (!far) return;
-  const int i = __ffs(far) - 1;
-  const int b = __shfl_sync(0xffffffffu, mine.x, i), hc = __shfl_sync(0xffffffffu, mine.y, i);
-  const int last = __shfl_sync(0xffffffffu, mine.z, i), head = __shfl_sync(0xffffffffu, mine.w, i);
-  const int mid = __shfl_sync(0xffffffffu, mid_mine, i);
-  // parts in line order: the tail slot of the first worker, the tail slots of the first
-  // workers of the CTAs behind it, the head slot of the last worker if its run goes on
-  const int parts = 1 + mid + head;
-  auto part = [&](int x) -> const float* {
-    const int64_t s = x == 0     ? slot_of(first_worker + i, 0)
-                      : x <= mid ? slot_of(static_cast<int64_t>(blockIdx.x + x) * kWarps, 0)
-                                 : slot_of(last, 1);
-    return a.ws + s * S::kSlot;
-  };
-  for (int at = blockIdx.y; at < NT * S::kBlocks; at += gridDim.y) {
-    const int nt = at / S::kBlocks;
-    Joined j;
-    for (int x0 = warp; x0 < parts; x0 += kJoinWarps * kJoinBatch) {
-      float2 m[kJoinBatch], l[kJoinBatch];
-      float4 v[kJoinBatch];
+  for (; far; far &= far - 1) {
+    const int i = __ffs(far) - 1;
+    const int b = __shfl_sync(0xffffffffu, mine.x, i), hc = __shfl_sync(0xffffffffu, mine.y, i);
+    const int last = __shfl_sync(0xffffffffu, mine.z, i);
+    const int head = __shfl_sync(0xffffffffu, mine.w, i);
+    const int mid = __shfl_sync(0xffffffffu, mid_mine, i);
+    const int parts = 1 + mid + head;
+    auto part = [&](int x) -> const float* {  // in line order
+      const int run = x == 0 ? first + i : x > mid ? last
+                      : kClaim ? first + i + x : (static_cast<int>(blockIdx.x) + x) * kWarps;
+      return a.ws.slot(run, x > mid ? 1 : 0, S::kSlot);
+    };
+    for (int at = blockIdx.y; at < NT * S::kBlocks; at += gridDim.y) {
+      const int nt = at / S::kBlocks;
+      Joined j;
+      for (int x0 = warp; x0 < parts; x0 += kJoinWarps * kJoinBatch) {
+        float2 m[kJoinBatch], l[kJoinBatch];
+        float4 v[kJoinBatch];
 #pragma unroll
-      for (int u = 0; u < kJoinBatch; ++u) {  // all loads first; absent parts weigh nothing
-        const int x = x0 + u * kJoinWarps;
-        const float* p = part(min(x, parts - 1));
-        m[u] = *reinterpret_cast<const float2*>(p + S::kOut + nt * 8 + 2 * c);
-        l[u] = *reinterpret_cast<const float2*>(p + S::kOut + NT * 8 + nt * 8 + 2 * c);
-        v[u] = reinterpret_cast<const float4*>(p)[at * 32 + lane];
+        for (int u = 0; u < kJoinBatch; ++u) {  // all loads first; absent parts are left out
+          const float* p = part(min(x0 + u * kJoinWarps, parts - 1));
+          m[u] = *reinterpret_cast<const float2*>(p + S::kOut + nt * 8 + 2 * c);
+          l[u] = *reinterpret_cast<const float2*>(p + S::kOut + NT * 8 + nt * 8 + 2 * c);
+          v[u] = reinterpret_cast<const float4*>(p)[at * 32 + lane];
+        }
+#pragma unroll
+        for (int u = 0; u < kJoinBatch; ++u)
+          if (x0 + u * kJoinWarps < parts) j.add(m[u].x, m[u].y, l[u].x, l[u].y, v[u]);
       }
+      s_acc[warp][lane] = j.acc;
+      s_ml[warp][lane] = make_float4(j.top0, j.top1, j.sum0, j.sum1);
+      __syncthreads();
+      if (warp == 0) {
+        Joined all;
 #pragma unroll
-      for (int u = 0; u < kJoinBatch; ++u)
-        if (x0 + u * kJoinWarps < parts) j.add(m[u].x, m[u].y, l[u].x, l[u].y, v[u]);
+        for (int w = 0; w < kJoinWarps; ++w)
+          all.add(s_ml[w][lane].x, s_ml[w][lane].y, s_ml[w][lane].z, s_ml[w][lane].w,
+                  s_acc[w][lane]);
+        finish(all, b, hc, nt, at % S::kBlocks);
+      }
+      __syncthreads();
     }
-    s_acc[warp][lane] = j.acc;
-    s_ml[warp][lane] = make_float4(j.top0, j.top1, j.sum0, j.sum1);
-    __syncthreads();
-    if (warp == 0) {
-      Joined all;
-#pragma unroll
-      for (int w = 0; w < kJoinWarps; ++w)
-        all.add(s_ml[w][lane].x, s_ml[w][lane].y, s_ml[w][lane].z, s_ml[w][lane].w,
-                s_acc[w][lane]);
-      finish(all, b, hc, nt, at % S::kBlocks);
-    }
-    __syncthreads();
   }
 }
 
-// CTAs of the main kernel: one per SM, fewer where the longest possible line is shorter.
-template <int D, bool kE4m3, int NT>
-int64_t grid_of(const PagedArgs& a) {
-  using S = Shape<D, kE4m3, NT>;
-  const int64_t tiles =
-      (static_cast<int64_t>(a.max_len) + S::kTile - 1) / S::kTile * a.batch * a.hkv * a.chunks;
-  int64_t ctas = std::min<int64_t>(sm_count(), kMaxWorkers / S::kWarps);
-  return std::max<int64_t>(1, std::min(ctas, (tiles + S::kWarps - 1) / S::kWarps));
+// Query heads that share a segment: 8, or 16 for wider groups, which halves the K and V
+// traffic of their segments (head_dim 256 keeps 8: accumulators of 16 would not fit the
+// registers).
+int heads_per_segment(int group, int head_dim) { return group > 8 && head_dim <= 128 ? 16 : 8; }
+
+// How a call is spread, from its sizes and the longest lengths that its table allows.
+struct Spread {
+  int64_t ctas;  // one per SM, fewer where the longest possible line is shorter
+  int64_t runs;  // runs that the workspace has room for
+  bool claim;    // runs are claimed as warps come free (see Cut)
+};
+Spread spread_of(int64_t batch, int hkv, int group, int head_dim, bool e4m3, int64_t max_len) {
+  const int row = head_dim * (e4m3 ? 1 : 2), tile = row <= 192 ? 2 * kSub : kSub;
+  const int warps = head_dim == 256 && !e4m3 ? 4 : 8;
+  const int per = heads_per_segment(group, head_dim);
+  const int64_t tiles = (max_len + tile - 1) / tile * batch * hkv * ((group + per - 1) / per);
+  Spread s;
+  s.ctas = std::max<int64_t>(
+      1, std::min<int64_t>(std::min<int64_t>(sm_count(), kMaxWorkers / warps),
+                           (tiles + warps - 1) / warps));
+  const int64_t workers = s.ctas * warps;
+  s.claim = tiles >= workers * kLeastClaimed && batch <= kCutBatch;
+  s.runs = s.claim ? workers * (1 + kSmall) : workers;
+  return s;
 }
 
 template <int D, bool kE4m3, int NT>
 void launch(PagedArgs a, cudaStream_t st) {
   using S = Shape<D, kE4m3, NT>;
   a.chunks = (a.group + 8 * NT - 1) / (8 * NT);
+  const Spread sp = spread_of(a.batch, a.hkv, a.group, D, kE4m3, a.max_len);
+  a.ws.runs = sp.runs;
   static std::once_flag once[64];
   int dev = 0;
   cudaGetDevice(&dev);
   std::call_once(once[dev & 63], [] {
-    cudaFuncSetAttribute(paged_attn_kernel<D, kE4m3, NT>,
-                         cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::kSmem));
-    cudaFuncSetAttribute(paged_join_kernel<D, kE4m3, NT>,
-                         cudaFuncAttributePreferredSharedMemoryCarveout,
-                         cudaSharedmemCarveoutMaxShared);
+    constexpr int smem = static_cast<int>(S::kSmem);
+    cudaFuncSetAttribute(paged_attn_kernel<D, kE4m3, NT, false>,
+                         cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaFuncSetAttribute(paged_attn_kernel<D, kE4m3, NT, true>,
+                         cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   });
-  const unsigned ctas = static_cast<unsigned>(grid_of<D, kE4m3, NT>(a));
-  launch_pdl(paged_attn_kernel<D, kE4m3, NT>, dim3(ctas), dim3(S::kWarps * 32), S::kSmem, st, a);
-  launch_pdl(paged_join_kernel<D, kE4m3, NT>, dim3(ctas, std::min(kJoinY, NT * S::kBlocks)),
-             dim3(kJoinWarps * 32), 0, st, a);
+  prefer_max_shared<paged_join_kernel<D, kE4m3, NT, false>>();
+  prefer_max_shared<paged_join_kernel<D, kE4m3, NT, true>>();
+  prefer_max_shared<paged_cut_kernel>();
+  const unsigned ctas = static_cast<unsigned>(sp.ctas);
+  const dim3 threads(S::kWarps * 32), joins(static_cast<unsigned>(sp.runs / S::kWarps),
+                                            std::min(kJoinY, NT * S::kBlocks));
+  if (sp.claim) {
+    launch_pdl(paged_cut_kernel, dim3(kCutCtas), dim3(kCutThreads), a.batch * sizeof(int), st, a,
+               D, S::kTile, static_cast<int>(ctas) * S::kWarps);
+    launch_pdl(paged_attn_kernel<D, kE4m3, NT, true>, dim3(ctas), threads, S::kSmem, st, a);
+    launch_pdl(paged_join_kernel<D, kE4m3, NT, true>, joins, dim3(kJoinWarps * 32), 0, st, a);
+  } else {
+    launch_pdl(paged_attn_kernel<D, kE4m3, NT, false>, dim3(ctas), threads, S::kSmem, st, a);
+    launch_pdl(paged_join_kernel<D, kE4m3, NT, false>, joins, dim3(kJoinWarps * 32), 0, st, a);
+  }
 }
 
-// Up to 8 query heads per KV head use one column tile; wider groups two, which halves the
-// K and V traffic of their segments (head_dim 256 keeps one: its accumulators of two would
-// not fit the registers).
 template <int D>
 void launch_d(const PagedArgs& a, bool e4m3, cudaStream_t st) {
   if constexpr (D <= 128) {
-    if (a.group > 8) {
+    if (heads_per_segment(a.group, D) == 16) {
       if (e4m3) launch<D, true, 2>(a, st);
       else launch<D, false, 2>(a, st);
       return;
@@ -928,13 +1098,15 @@ void launch_d(const PagedArgs& a, bool e4m3, cudaStream_t st) {
 
 using namespace umic;
 
-extern "C" size_t umic_paged_attention_workspace_bytes(int32_t hq, int32_t hkv,
-                                                       int32_t head_dim) {
-  if (hq <= 0 || hkv <= 0 || head_dim <= 0) return 0;
-  // per warp: two partial results (O, m, l of its query heads) and a split record
-  const size_t heads = hq / hkv > 8 && head_dim <= 128 ? 16 : 8;
-  const size_t workers = static_cast<size_t>(std::min<int64_t>(sm_count() * 8, kMaxWorkers));
-  return workers * (2 * heads * (head_dim + 2) * sizeof(float) + sizeof(Split));
+extern "C" size_t umic_paged_attention_workspace_bytes(int64_t batch, int32_t hq, int32_t hkv,
+                                                       int32_t head_dim, int64_t max_pages,
+                                                       int64_t page_size, int cache_dtype) {
+  if (batch <= 0 || hq <= 0 || hkv <= 0 || head_dim <= 0 || max_pages < 0 || page_size <= 0 ||
+      hq / hkv == 0)
+    return 0;
+  const Spread s = spread_of(batch, hkv, hq / hkv, head_dim, cache_dtype == UMIC_DTYPE_E4M3,
+                             max_pages * page_size);
+  return Space::bytes(s.runs, heads_per_segment(hq / hkv, head_dim) * (head_dim + 2));
 }
 
 extern "C" int umic_paged_attention(
@@ -978,10 +1150,11 @@ extern "C" int umic_paged_attention(
   if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out) ||
       q_sb % 8 || q_sh % 8 || o_sb % 8 || o_sh % 8 || pg_sp % pe || pg_sh % pe || pg_ss % pe)
     return fail(UMIC_ERR_ALIGNMENT, "%s: 16-byte alignment of bases / strides", me);
-  if (!workspace || !aligned16(workspace) ||
-      workspace_bytes < umic_paged_attention_workspace_bytes(hq, hkv, head_dim))
+  const size_t need = umic_paged_attention_workspace_bytes(batch, hq, hkv, head_dim, max_pages,
+                                                           page_size, cache_dtype);
+  if (!workspace || !aligned16(workspace) || workspace_bytes < need)
     return fail(UMIC_ERR_INVALID_ARG, "%s: workspace of %zu bytes (%zu needed, 16-byte aligned)",
-                me, workspace_bytes, umic_paged_attention_workspace_bytes(hq, hkv, head_dim));
+                me, workspace_bytes, need);
   uint32_t* err = device_error_word();
   if (!err) return fail(UMIC_ERR_DEVICE, "%s: no device error word", me);
   const bool e4m3 = cache_dtype == UMIC_DTYPE_E4M3;
@@ -997,7 +1170,7 @@ extern "C" int umic_paged_attention(
   a.out = static_cast<__nv_bfloat16*>(out);
   a.lse = lse;
   a.err = err;
-  a.ws = static_cast<float*>(workspace);
+  a.ws.base = static_cast<char*>(workspace);
   a.q_sb = q_sb; a.q_sh = q_sh; a.o_sb = o_sb; a.o_sh = o_sh;
   a.pg_sp = pg_sp * es; a.pg_sh = pg_sh * es; a.pg_ss = pg_ss * es;
   a.table_stride = table_stride;

@@ -81,7 +81,8 @@ _SIGNATURES: dict[str, list] = {
                              _c_i64, _c_int, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p,
                              _c_i64, _c_i64, _c_p, _c_i64, _c_i32, _c_i32, _c_i32, _c_f32, _c_p,
                              _c_size, _c_p],
-    "umic_paged_attention_workspace_bytes": [_c_i32, _c_i32, _c_i32],
+    "umic_paged_attention_workspace_bytes": [_c_i64, _c_i32, _c_i32, _c_i32, _c_i64, _c_i64,
+                                             _c_int],
     "umic_gemm": [_c_p, _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_i64, _c_p, _c_i64, _c_i64, _c_i64,
                   _c_i64, _c_int, _c_p],
     "umic_gemm_ws": [_c_p, _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_i64, _c_p, _c_i64, _c_i64,

@@ -268,7 +268,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     # its own workspace for every call: calls on several streams, and graphs captured
     # apart, never share one
     _lib._ensure_device(dev)
-    need = _lib.lib().umic_paged_attention_workspace_bytes(hq, hk, d)
+    need = _lib.lib().umic_paged_attention_workspace_bytes(
+        b, hq, hk, d, block_table.shape[1], page, dt)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     _lib.call("umic_paged_attention", dev, q.data_ptr(), q.stride(0), q.stride(1),
               k_pages.data_ptr(), v_pages.data_ptr(), *k_pages.stride()[:3], p, page, dt,
