@@ -19,9 +19,9 @@
 //   m, l, P        running maximum and sum of each head, fp32, base 2
 //   O^T += V^T P   V through transposing ldmatrix, P transposed in registers
 // P is fp32 split into a bf16 value and its bf16 remainder (two products, weights held to
-// 2^-17): the tensor pipe has the time. e4m3 pages are widened to fp16 in registers, which
-// holds them exactly; q is scaled by a power of two to stay inside fp16 and P by 2^14 so
-// that small weights stay normal, rounded to 2^-12.
+// 2^-17): the tensor pipe has the time. e4m3
+// pages are widened to fp16 in registers, which holds them exactly; q is scaled by a power
+// of two to stay inside fp16 and P by 2^15 so that small weights stay normal, to 2^-12.
 //
 // Join. A warp whose run covers a whole segment writes its rows. Otherwise it has partial
 // (m, l, O): neighbours of one CTA that share a segment join through shared memory, and
@@ -34,15 +34,13 @@
 #include <cmath>
 
 #include "common.cuh"
-#include "mma_frag.cuh"
 
 namespace umic {
 namespace {
 
 constexpr int kSub = 16;              // tokens per subtile: rows of one mma, within one page
-constexpr float kF16Shift = 14.f;     // e4m3 path: weights are held as 2^14 p
+constexpr float kF16Shift = 15.f;     // e4m3 path: weights are held as 2^15 p
 constexpr int kSmemBudget = 216 * 1024;
-constexpr int64_t kMaxWorkers = 2048;  // warps of the main kernel, bounds the workspace
 
 // A split segment, left by the run that holds its first tile for the joining kernel.
 struct Split {
@@ -52,23 +50,17 @@ struct Split {
   int32_t head;  // 1: that run goes on behind the segment
 };
 
-// The workspace: a header, where each run begins, the splits, and two partial results for
-// each run (0: of its last segment, 1: of its first if that is another).
-struct Header {
-  int32_t total, big, runs, next;  // tiles of the line and of its big runs; runs; runs claimed
-  int32_t pad[12];
-};
+// The workspace: the splits, and two partial results for each warp's run (0: of its last
+// segment, 1: of its first if that is another).
 struct Space {
   char* base;
   int64_t runs;  // room for
-  __host__ __device__ Header* header() const { return reinterpret_cast<Header*>(base); }
-  __host__ __device__ int4* starts() const { return reinterpret_cast<int4*>(base + sizeof(Header)); }
-  __host__ __device__ Split* splits() const { return reinterpret_cast<Split*>(starts() + runs); }
+  __host__ __device__ Split* splits() const { return reinterpret_cast<Split*>(base); }
   __host__ __device__ float* slot(int64_t run, int head, int floats) const {
     return reinterpret_cast<float*>(splits() + runs) + (run * 2 + head) * floats;
   }
   static constexpr size_t bytes(int64_t runs, int64_t floats) {
-    return sizeof(Header) + runs * (sizeof(int4) + sizeof(Split) + 2 * floats * sizeof(float));
+    return runs * (sizeof(Split) + 2 * floats * sizeof(float));
   }
 };
 
@@ -83,29 +75,49 @@ struct PagedArgs {
   Space ws;
   int64_t q_sb, q_sh, pg_sp, pg_sh, pg_ss;  // pg_* in bytes
   int64_t table_stride, num_pages, o_sb, o_sh;
-  int32_t max_len, page_size, hq, hkv, batch, group, chunks;  // chunks: segments per KV head
+  int32_t max_len, max_pages, page_size, hq, hkv, batch, group, chunks;  // chunks: segments per KV head
   float scale_log2;
 };
+
+constexpr int subtiles(int d, bool e4m3) { return d * (e4m3 ? 1 : 2) <= 192 ? 2 : 1; }
+// Warps of a CTA. bf16: 8, of whose ring of three 8 KB tiles two fill while one is used
+// (head_dim 256: 4, whose accumulators fit the registers). e4m3: the work of widening,
+// twice per byte, wants 12 to hide its latencies (256 requests of up to 4096 tokens: 217 us
+// against 240 with 8), unless two column tiles' accumulators leave room for 8 only.
+constexpr int warps_per_cta(int d, bool e4m3, int per) {
+  return e4m3 ? (d >= 128 && per > 8 ? 8 : 12) : d == 256 ? 4 : 8;
+}
 
 // Shapes of one instantiation.
 template <int D, bool kE4m3, int NT>
 struct Shape {
   static constexpr int kRow = D * (kE4m3 ? 1 : 2);                   // bytes of a token's row
-  static constexpr int kPitch = kRow + ((kRow / 16) % 2 ? 0 : 16);  // odd count of 16 B: no
-                                                                    // bank conflicts
-  // Rows of up to 192 bytes go two subtiles a tile: the running maximum and its shuffles
+  // Rows in shared memory, so that eight rows' same 16 bytes fall in different banks: whole
+  // 128-byte lines with their 16-byte pieces exchanged (piece p of row r at p ^ r % 8), else
+  // padded to an odd count of pieces. (Padding 256-byte rows too was 6 per cent slower:
+  // copies then straddle lines.)
+  static constexpr bool kSwizzle = kRow % 128 == 0;
+  static constexpr int kPitch = kSwizzle ? kRow : kRow + ((kRow / 16) % 2 ? 0 : 16);
+  __device__ static uint32_t piece(int row, int p) {
+    return row * kPitch + (kSwizzle ? p ^ (row & 7) : p) * 16;
+  }
+  // the piece `bytes` further on in a row, from one whose number has those bits clear
+  __device__ static uint32_t along(uint32_t at, int bytes) {
+    return kSwizzle ? at ^ bytes : at + bytes;
+  }
+  // Two subtiles a tile for rows of up to 192 bytes: the running maximum and its shuffles
   // cost a tile the same whatever it holds.
-  static constexpr int MT = kRow <= 192 ? 2 : 1;
+  static constexpr int MT = subtiles(D, kE4m3);
   static constexpr int kTile = kSub * MT;                           // tokens per tile
   static constexpr int kSubBytes = 2 * kSub * kPitch;               // K, then V
   static constexpr int kTileBytes = MT * kSubBytes;
-  static constexpr int kWarps = D == 256 && !kE4m3 ? 4 : 8;
+  static constexpr int kWarps = warps_per_cta(D, kE4m3, 8 * NT);
   static constexpr int kFit = kSmemBudget / (kWarps * kTileBytes);
   static constexpr int kStages = kFit < 6 ? kFit : 6;
   static constexpr int kBlocks = D / 16;                            // 16-dim blocks
   static constexpr int kOut = NT * kBlocks * 128;                   // floats of one partial O
   static constexpr int kSlot = kOut + NT * 16;                      // + m and l of 8 * NT heads
-  static constexpr size_t kSmem = static_cast<size_t>(kWarps) * kStages * kTileBytes;
+  static constexpr size_t kSmem = static_cast<size_t>(kWarps) * kStages * kTileBytes + 512;
   static_assert(kStages >= 2, "one tile in use, one in flight");
   static_assert(kStages * kTileBytes >= kSlot * 4, "a partial result fits its warp's ring");
 };
@@ -117,6 +129,9 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool t
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
                "r"(there ? 16 : 0)
                : "memory");
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -152,10 +167,18 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
+// Not volatile: products of different accumulators may be moved past one another, so that
+// a chain's next product need not wait for the last.
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
+      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                         uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
       "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -173,11 +196,21 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-// two e4m3 values (low byte first) as fp16, exactly
-__device__ __forceinline__ uint32_t widen(uint32_t two) {
-  const __half2_raw h =
-      __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two & 0xffffu), __NV_E4M3);
-  return static_cast<uint32_t>(h.x) | static_cast<uint32_t>(h.y) << 16;
+// Four e4m3 values as fp16 pairs (bytes 0, 2 and bytes 1, 3), times kWide, exactly. The
+// seven bits below the sign, put three places higher in fp16, are the value times 2^-8,
+// subnormals included; the product with 2^8 kWide has 4 + 6 bits, is normal, and sends the
+// NaN code (which the shift makes 480 * 2^-8) over the largest fp16 to infinity, so that a
+// NaN in K or V still reaches its rows. Nine instructions, five of them on the ALU pipe,
+// which the conversion instruction would fill.
+constexpr float kWide = 140.f;
+__device__ __forceinline__ void widen4(uint32_t r, uint32_t& even, uint32_t& odd) {
+  const uint32_t e = ((r * 256u) & 0x80008000u) | ((r * 128u) & 0x3f803f80u);
+  const uint32_t o = (r & 0x80008000u) | ((r >> 1) & 0x3f803f80u);
+  const __half2 up = __float2half2_rn(256.f * kWide);
+  const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&e), up);
+  const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&o), up);
+  even = *reinterpret_cast<const uint32_t*>(&x);
+  odd = *reinterpret_cast<const uint32_t*>(&y);
 }
 
 __device__ __forceinline__ int clamped_len(const PagedArgs& a, int b) {
@@ -193,29 +226,6 @@ struct Line {
   __device__ int run_of(int x) const {
     const int cut = longer * (base + 1);
     return x < cut ? x / (base + 1) : longer + (x - cut) / base;
-  }
-};
-
-// Which runs a line is cut into when they are claimed as warps come free. At full HBM load
-// the SMs do not get equal shares (measured per SM on a 2 GB line: 470 to 650 thousand
-// cycles for equal runs, by their place on the chip), so each warp first has a run of
-// 11 / 16 of its equal share and the rest is cut into kSmall runs per warp: the warps that
-// are ahead take more of them. Which runs there are depends on the lengths alone, so sums
-// are taken alike whoever computes them.
-constexpr int kSmall = 4;
-constexpr int kLeastClaimed = 32;  // tiles a warp from which on the line is cut so
-template <bool kClaim>
-struct Cut {
-  Line big, small;
-  int big_tiles, workers;
-  __device__ Cut(int total, int big_total, int n)
-      : big(big_total, n), small(kClaim ? total - big_total : 0, kClaim ? n * kSmall : 1),
-        big_tiles(big_total), workers(n) {}
-  __device__ int begin(int r) const {
-    return !kClaim || r <= workers ? big.begin(r) : big_tiles + small.begin(r - workers);
-  }
-  __device__ int run_of(int x) const {
-    return !kClaim || x < big_tiles ? big.run_of(x) : workers + small.run_of(x - big_tiles);
   }
 };
 
@@ -253,7 +263,7 @@ struct Rows {
     }
   }
   __device__ static float inverse(const PagedArgs& a, int hc, float l) {
-    const float unit = kE4m3 && a.v_scale ? a.v_scale[hc / a.chunks] : 1.f;
+    const float unit = kE4m3 ? (a.v_scale ? a.v_scale[hc / a.chunks] : 1.f) / kWide : 1.f;
     return l == 0.f ? 0.f : unit / l;
   }
   __device__ static void store_lse(const PagedArgs& a, int b, int hc, int nt, float m0, float l0,
@@ -295,68 +305,7 @@ __device__ __forceinline__ int block_sums(int mine, int* s_warp_sum, int* total)
   return upto;
 }
 
-// Zero rows of the requests without tokens, dealt to the CTAs.
-__device__ __forceinline__ void zero_empty(const PagedArgs& a, int d) {
-  for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
-    if (clamped_len(a, b) > 0) continue;
-    for (int i = threadIdx.x; i < a.hq * (d / 8); i += blockDim.x)
-      st_vec(a.out + b * a.o_sb + i / (d / 8) * a.o_sh + i % (d / 8) * 8, make_uint4(0, 0, 0, 0));
-    if (a.lse)
-      for (int h = threadIdx.x; h < a.hq; h += blockDim.x)
-        a.lse[static_cast<int64_t>(b) * a.hq + h] = -INFINITY;
-  }
-}
-
-// Cuts the line for claimed runs: the header and where each run begins. Every CTA scans
-// the lengths and places its share of the runs.
-constexpr int kCutThreads = 512, kCutCtas = 8, kCutBatch = 8192;
-__global__ void __launch_bounds__(kCutThreads) paged_cut_kernel(PagedArgs a, int d, int tile,
-                                                                int workers) {
-  extern __shared__ int s_first[];  // tile of the line at which each request begins
-  __shared__ int s_warp_sum[kCutThreads / 32];
-  allow_dependent_launch();
-  wait_prerequisite();
-  const int hcs = a.hkv * a.chunks;
-  const int per = (a.batch + kCutThreads - 1) / kCutThreads;
-  const int b0 = min(a.batch, static_cast<int>(threadIdx.x) * per), b1 = min(a.batch, b0 + per);
-  int mine = 0;
-  for (int b = b0; b < b1; ++b) {
-    const int n = a.lens[b];
-    if (blockIdx.x == 0 && (n < 0 || n > a.max_len)) atomicOr(a.err, UMIC_DEVERR_BAD_PAGE);
-    s_first[b] = mine;
-    mine += (max(0, min(n, a.max_len)) + tile - 1) / tile;
-  }
-  int total;
-  const int upto = block_sums<kCutThreads / 32>(mine, s_warp_sum, &total);
-  for (int b = b0; b < b1; ++b) s_first[b] = (s_first[b] + upto) * hcs;
-  total *= hcs;
-  __syncthreads();
-  workers = min(workers, total);
-  const bool claimed = total >= workers * kLeastClaimed;
-  const int big = claimed ? total / 16 * 11 : total;
-  const int runs = claimed ? workers * (1 + kSmall) : workers;
-  if (blockIdx.x == 0 && threadIdx.x == 0) {
-    Header* h = a.ws.header();
-    h->total = total;
-    h->big = big;
-    h->runs = runs;
-    h->next = workers;
-  }
-  const Cut<true> cut(total, big, max(workers, 1));
-  for (int r = blockIdx.x * kCutThreads + threadIdx.x; r < runs; r += gridDim.x * kCutThreads) {
-    const int at = cut.begin(r);
-    int lo = 0, hi = a.batch;  // the last request that begins at or before `at`: it has tiles
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (s_first[mid] <= at) lo = mid; else hi = mid;
-    }
-    const int len = clamped_len(a, lo), tiles = (len + tile - 1) / tile, in = at - s_first[lo];
-    a.ws.starts()[r] = make_int4(lo, in / tiles, in % tiles, len);
-  }
-  zero_empty(a, d);
-}
-
-template <int D, bool kE4m3, int NT, bool kClaim>
+template <int D, bool kE4m3, int NT>
 __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
     paged_attn_kernel(PagedArgs a) {
   using S = Shape<D, kE4m3, NT>;
@@ -364,12 +313,12 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
   constexpr int kWarps = S::kWarps, kStages = S::kStages, kBlocks = S::kBlocks;
   constexpr int kThreads = kWarps * 32, MT = S::MT, kTile = S::kTile;
   auto tiles_of = [](int len) { return (len + kTile - 1) / kTile; };
-  extern __shared__ __align__(16) char ring_mem[];
+  extern __shared__ char smem[];
+  char* const ring_mem = smem + (-smem_addr(smem) & 511u);  // rows lie on their own size
   // request (-1: no more tiles), segment, valid rows (a byte per subtile) and flags, tiles
   // left of the segment
   __shared__ int4 s_info[kWarps][kStages];
-  constexpr int kSegFirst = 1 << 16, kRunFirst = 1 << 17, kRunLast = 1 << 18;
-  __shared__ int s_run[kClaim ? kWarps : 1][kStages];
+  constexpr int kRunLast = 1 << 16;
   __shared__ int4 s_begin[kWarps];          // request, segment, tile and request length at a
                                             // warp's start
   __shared__ int s_warp_sum[kWarps];
@@ -382,95 +331,110 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
   const int hcs = a.hkv * a.chunks;  // segments per request
 
   const int first_worker = static_cast<int>(blockIdx.x) * kWarps;
-  int total, workers;
-  if constexpr (!kClaim) {
-    // ---- the line of tiles, and where each warp's run begins on it
-    const int per = (a.batch + kThreads - 1) / kThreads;
-    const int b0 = min(a.batch, static_cast<int>(threadIdx.x) * per), b1 = min(a.batch, b0 + per);
-    int mine = 0, first_len = 0;
-    for (int b = b0; b < b1; ++b) {
-      const int n = a.lens[b];
-      if (blockIdx.x == 0 && (n < 0 || n > a.max_len)) atomicOr(a.err, UMIC_DEVERR_BAD_PAGE);
-      const int len = max(0, min(n, a.max_len));
-      if (b == b0) first_len = len;
-      mine += tiles_of(len);
-    }
-    const int upto = block_sums<kWarps>(mine, s_warp_sum, &total);
-    total *= hcs;
-    workers = min(static_cast<int>(gridDim.x) * kWarps, total);
-    const Line line(total, max(workers, 1));
-    if (mine > 0 && first_worker < workers && line.begin(first_worker + kWarps) > upto * hcs) {
-      for (int w = 0; w < kWarps && first_worker + w < workers; ++w) {
-        int at = line.begin(first_worker + w) - upto * hcs;
-        if (at < 0 || at >= mine * hcs) continue;
-        int len = first_len;
-        for (int b = b0;; len = clamped_len(a, ++b)) {
-          const int tiles = tiles_of(len);
-          if (at < tiles * hcs) {
-            s_begin[w] = make_int4(b, at / tiles, at % tiles, len);
-            break;
-          }
-          at -= tiles * hcs;
+  // ---- the line of tiles, and where each warp's run begins on it
+  const int per = (a.batch + kThreads - 1) / kThreads;
+  const int b0 = min(a.batch, static_cast<int>(threadIdx.x) * per), b1 = min(a.batch, b0 + per);
+  int mine = 0, first_len = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int n = a.lens[b];
+    if (blockIdx.x == 0 && (n < 0 || n > a.max_len)) atomicOr(a.err, UMIC_DEVERR_BAD_PAGE);
+    const int len = max(0, min(n, a.max_len));
+    if (b == b0) first_len = len;
+    mine += tiles_of(len);
+  }
+  int total;
+  const int upto = block_sums<kWarps>(mine, s_warp_sum, &total);
+  total *= hcs;
+  const int workers = min(static_cast<int>(gridDim.x) * kWarps, total);
+  const Line line(total, max(workers, 1));
+  if (mine > 0 && first_worker < workers && line.begin(first_worker + kWarps) > upto * hcs) {
+    for (int w = 0; w < kWarps && first_worker + w < workers; ++w) {
+      int at = line.begin(first_worker + w) - upto * hcs;
+      if (at < 0 || at >= mine * hcs) continue;
+      int len = first_len;
+      for (int b = b0;; len = clamped_len(a, ++b)) {
+        const int tiles = tiles_of(len);
+        if (at < tiles * hcs) {
+          s_begin[w] = make_int4(b, at / tiles, at % tiles, len);
+          break;
         }
+        at -= tiles * hcs;
       }
     }
-    zero_empty(a, D);
-    __syncthreads();
-  } else {
-    total = a.ws.header()->total;
-    workers = min(static_cast<int>(gridDim.x) * kWarps, total);
   }
+  // requests without tokens, dealt to the CTAs: zeros
+  for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
+    if (clamped_len(a, b) > 0) continue;
+    for (int i = threadIdx.x; i < a.hq * (D / 8); i += kThreads)
+      st_vec(a.out + b * a.o_sb + i / (D / 8) * a.o_sh + i % (D / 8) * 8, make_uint4(0, 0, 0, 0));
+    if (a.lse)
+      for (int h = threadIdx.x; h < a.hq; h += kThreads)
+        a.lse[static_cast<int64_t>(b) * a.hq + h] = -INFINITY;
+  }
+  __syncthreads();
 
   const int worker = first_worker + warp;
-  const int runs = kClaim ? a.ws.header()->runs : workers;
-  const Cut<kClaim> cut(total, kClaim ? a.ws.header()->big : total, max(workers, 1));
+  int left = worker < workers ? line.begin(worker + 1) - line.begin(worker) : 0;  // to copy
+
   char* const ring = ring_mem + static_cast<size_t>(warp) * kStages * S::kTileBytes;
   const uint32_t ring_addr = smem_addr(ring);
 
   // ---- loader: the next tile to copy. Pages are looked up one tile ahead of their copies.
   int lb = 0, lhc = 0, lt = 0, ltiles = 0, lpi = 0, loff = 0, llen = 0;
   int page_id[MT], page_off[MT];
-  const int32_t* row_of_table = a.table;
+  // A lane holds one of 32 consecutive table entries, and the next 32, the row's first 32
+  // (for the next head) and the next request's first 32 and length are under way: under
+  // full load a dependent look-up takes microseconds.
+  int entries = 0, entries_next = 0, entries_first = 0, other_entries = 0, other_len = 0;
+  auto entry = [&](int b, int i) {
+    return b < a.batch && i < a.max_pages ? a.table[b * a.table_stride + i] : 0;
+  };
+  auto fetch_other = [&]() {
+    other_entries = entry(lb + 1, lane);
+    other_len = lb + 1 < a.batch ? clamped_len(a, lb + 1) : 0;
+  };
   auto look_up = [&]() {  // pages of tile lt; steps (lpi, loff) behind it
 #pragma unroll
     for (int u = 0; u < MT; ++u) {
       page_off[u] = loff;
-      page_id[u] = u == 0 || lt * kTile + u * kSub < llen ? row_of_table[lpi] : 0;
+      page_id[u] = __shfl_sync(0xffffffffu, entries, lpi & 31);
       if ((loff += kSub) == a.page_size) {
         loff = 0;
-        ++lpi;
+        if ((++lpi & 31) == 0) {
+          entries = entries_next;
+          entries_next = entry(lb, lpi + 32 + lane);
+        }
       }
     }
   };
-  // the run being copied, its tiles still to copy, and the run after it
-  int lrun = worker, left = 0, fresh = 0, next_run = 0;
-  int4 next_start;
-  auto start_run = [&](const int4& st) {
-    left = cut.begin(lrun + 1) - cut.begin(lrun);
-    fresh = kRunFirst;
-    lb = st.x;
-    lhc = st.y;
-    lt = st.z;
-    llen = st.w;
+  auto touch_q = [&]() {  // a new segment's q into L1, while its first tiles come
+    const int n = R::heads(a, lhc);
+    const char* q = reinterpret_cast<const char*>(
+        a.q + lb * a.q_sb + static_cast<int64_t>(R::head0(a, lhc)) * a.q_sh);
+    constexpr int kLines = (2 * D + 127) / 128;
+    for (int i = lane; i < n * kLines; i += 32)
+      asm volatile("prefetch.global.L1 [%0];" ::"l"(q + i / kLines * a.q_sh * 2 + i % kLines * 128));
+  };
+  const int4 start = left > 0 ? s_begin[warp] : make_int4(0, 0, 0, 0);
+  if (left > 0) {
+    lb = start.x;
+    lhc = start.y;
+    lt = start.z;
+    llen = start.w;
     ltiles = tiles_of(llen);
-    row_of_table = a.table + lb * a.table_stride;
     lpi = lt * kTile / a.page_size;
     loff = lt * kTile - lpi * a.page_size;
+    entries = entry(lb, (lpi & ~31) + lane);
+    entries_next = entry(lb, (lpi & ~31) + 32 + lane);
+    entries_first = entry(lb, lane);
+    fetch_other();
     look_up();
-    if constexpr (kClaim) {  // the next one is claimed now and needed a run later
-      if (lane == 0) next_run = atomicAdd(&a.ws.header()->next, 1);
-      next_run = __shfl_sync(0xffffffffu, next_run, 0);
-      if (next_run < runs) next_start = a.ws.starts()[next_run];
-    }
-  };
-  int4 start = make_int4(0, 0, 0, 0);
-  if (worker < workers) {
-    start = kClaim ? a.ws.starts()[worker] : s_begin[warp];
-    start_run(start);
   }
   constexpr int kCols = S::kRow / 16;  // 16-byte pieces of a row
   constexpr int kCopies = (kSub * kCols + 31) / 32;
   const bool dense = a.pg_ss == S::kRow;  // a page's rows of a head lie one behind the other
+  constexpr bool kEven = 32 % kCols == 0;  // 32 lanes copy whole rows
+  const uint32_t lane_dst = S::piece(lane / kCols, lane % kCols);
   const int64_t v_minus_k = a.v_pages - a.k_pages;
   auto load = [&](int stage) {
     if (left > 0) {
@@ -488,16 +452,16 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
         rows_of |= rows << (8 * u);
         const char* k = a.k_pages + page * a.pg_sp + head_at + page_off[u] * a.pg_ss;
         const uint32_t dst = ring_addr + stage * S::kTileBytes + u * S::kSubBytes;
-        if (dense && rows == kSub) {
-          k += lane * 16;
-          const char* v = k + v_minus_k;
+        if (kEven && dense && rows == kSub) {  // immediate offsets from two pointers
+          const uint32_t to = dst + lane_dst;
+          const char* at_k = k + lane * 16;
+          const char* at_v = at_k + v_minus_k;
 #pragma unroll
           for (int i = 0; i < kCopies; ++i) {
-            const int x = i * 32 + lane;
-            const uint32_t to = dst + x / kCols * S::kPitch + x % kCols * 16;
-            if ((kSub * kCols) % 32 != 0 && x >= kSub * kCols) break;
-            cp_async16(to, k + i * 512, true);
-            cp_async16(to + kSub * S::kPitch, v + i * 512, true);
+            const int row = i * (32 / kCols);  // of lane 0
+            const uint32_t into = (S::kSwizzle ? to ^ ((row & 7) * 16) : to) + row * S::kPitch;
+            cp_async16(into, at_k + i * 512);
+            cp_async16(into + kSub * S::kPitch, at_v + i * 512);
           }
         } else {
           // rows behind the length are filled with zeros: a weight of 0 times what an
@@ -505,7 +469,7 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
 #pragma unroll
           for (int i = 0; i < kCopies; ++i) {
             const int x = i * 32 + lane, row = x / kCols;
-            const uint32_t to = dst + row * S::kPitch + x % kCols * 16;
+            const uint32_t to = dst + S::piece(row, x % kCols);
             if ((kSub * kCols) % 32 != 0 && x >= kSub * kCols) break;
             const char* at = k + row * a.pg_ss + x % kCols * 16;
             cp_async16(to, at, row < rows);
@@ -515,26 +479,29 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
       }
       --left;
       if (lane == 0) {
-        const int flags = fresh | (lt == 0 ? kSegFirst : 0) | (left == 0 ? kRunLast : 0);
-        s_info[warp][stage] = make_int4(lb, lhc, rows_of | flags, ltiles - lt);
-        if constexpr (kClaim) s_run[warp][stage] = lrun;
+        s_info[warp][stage] = make_int4(lb, lhc, rows_of | (left == 0 ? kRunLast : 0), ltiles - lt);
       }
-      fresh = 0;
       if (left > 0) {
         if (++lt == ltiles) {
           lt = lpi = loff = 0;
           if (++lhc == hcs) {
             lhc = 0;
-            do llen = clamped_len(a, ++lb);
-            while (llen == 0);
+            ++lb;
+            llen = other_len;
+            entries_first = other_entries;
+            if (llen == 0) {  // the requests behind an empty one are looked up in turn
+              do llen = clamped_len(a, ++lb);
+              while (llen == 0);
+              entries_first = entry(lb, lane);
+            }
             ltiles = tiles_of(llen);
-            row_of_table = a.table + lb * a.table_stride;
+            fetch_other();
           }
+          entries = entries_first;
+          entries_next = entry(lb, 32 + lane);
+          touch_q();
         }
         look_up();
-      } else if (kClaim && next_run < runs) {
-        lrun = next_run;
-        start_run(next_start);
       }
     } else if (lane == 0) {
       s_info[warp][stage].x = -1;
@@ -566,8 +533,8 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
         }
         fac[nt][0] = fac[nt][1] = a.scale_log2;
       } else {
-        // a lane's four bytes of a K row are dims 4c .. 4c + 3 of a block: q to match,
-        // scaled by the power of two of its largest value
+        // a lane's four bytes of a K row are dims 4c .. 4c + 3 of a block, widened as 4c,
+        // 4c + 2 and 4c + 1, 4c + 3: q to match, as fp16, scaled by the power of two of the row's largest
         uint2 raw[kBlocks];
         float top = 0.f;
 #pragma unroll
@@ -580,20 +547,20 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // 2^e <= top < 2^(e + 1); e kept where 2^-e is a normal number
-        const int e = top > 0.f && top < INFINITY
-                          ? max(-126, min(126, static_cast<int>(__float_as_uint(top) >> 23) - 127))
-                          : 0;
+        // 2^e <= top < 2^(e + 1); e kept where 2^e and 2^-e are normal numbers
+        const int e = max(-126, min(126, static_cast<int>(__float_as_uint(top) >> 23) - 127));
         const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-        const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+        // an infinity in q makes every score of its head infinite or NaN, and the row NaN
+        const float up = top < INFINITY ? __uint_as_float(static_cast<uint32_t>(127 + e) << 23)
+                                        : NAN;
 #pragma unroll
         for (int k = 0; k < kBlocks; ++k) {
           qf[nt][k][0] = pack_f16(__uint_as_float(raw[k].x << 16) * down,
-                                  __uint_as_float(raw[k].x & 0xffff0000u) * down);
-          qf[nt][k][1] = pack_f16(__uint_as_float(raw[k].y << 16) * down,
+                                  __uint_as_float(raw[k].y << 16) * down);
+          qf[nt][k][1] = pack_f16(__uint_as_float(raw[k].x & 0xffff0000u) * down,
                                   __uint_as_float(raw[k].y & 0xffff0000u) * down);
         }
-        const float f = a.scale_log2 * (a.k_scale ? a.k_scale[hc / a.chunks] : 1.f) * up;
+        const float f = a.scale_log2 * (a.k_scale ? a.k_scale[hc / a.chunks] : 1.f) / kWide * up;
         fac[nt][0] = __shfl_sync(0xffffffffu, f, 8 * c);
         fac[nt][1] = __shfl_sync(0xffffffffu, f, 8 * c + 4);
       }
@@ -606,44 +573,51 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
 
   auto tile = [&](int stage, int rows_of) {
     const uint32_t at0 = ring_addr + stage * S::kTileBytes;
-    // S^T: one accumulator per subtile, or two that share the chain of a single one
-    float s[NT][2][4];
+    // S^T in four accumulators, 4 / MT a subtile, to keep the chains of dependent products
+    // short
+    float s[NT][4][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[nt][0][j] = s[nt][1][j] = 0.f;
-    const uint32_t k_at = at0 + ((lane & 7) + (lane & 8)) * S::kPitch + (lane >> 4) * 16;
+      for (int x = 0; x < 4; ++x)
 #pragma unroll
-    for (int u = 0; u < MT; ++u) {
-      const uint32_t at = k_at + u * S::kSubBytes;
-      if constexpr (!kE4m3) {
+        for (int j = 0; j < 4; ++j) s[nt][x][j] = 0.f;
+    const uint32_t k_at = at0 + S::piece((lane & 7) + (lane & 8), lane >> 4);
+    if constexpr (!kE4m3) {
 #pragma unroll
-        for (int k = 0; k < kBlocks; ++k) {
-          uint32_t r[4];
-          ldsm4(r, at + k * 32);
+      for (int k = 0; k < kBlocks; ++k) {
+        uint32_t r[MT][4];
+#pragma unroll
+        for (int u = 0; u < MT; ++u) ldsm4(r[u], S::along(k_at + u * S::kSubBytes, k * 32));
+#pragma unroll
+        for (int u = 0; u < MT; ++u)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
-            mma16816(s[nt][MT == 2 ? u : k & 1], r[0], r[1], r[2], r[3], qf[nt][k][0],
-                     qf[nt][k][1]);
-        }
-      } else {
+            mma_bf16(s[nt][MT == 2 ? 2 * u + (k & 1) : k & 3], r[u], qf[nt][k][0], qf[nt][k][1]);
+      }
+    } else {
 #pragma unroll
-        for (int k = 0; k < kBlocks; k += 2) {
+      for (int k = 0; k < kBlocks; k += 2) {
+#pragma unroll
+        for (int u = 0; u < MT; ++u) {
           uint32_t r[4];
-          if (k + 1 < kBlocks) ldsm4(r, at + k * 16);
-          else ldsm2(r[0], r[1], at + k * 16);
+          const uint32_t at = S::along(k_at + u * S::kSubBytes, k * 16);
+          if (k + 1 < kBlocks) ldsm4(r, at);
+          else ldsm2(r[0], r[1], at);
 #pragma unroll
           for (int x = 0; x < 2 && k + x < kBlocks; ++x) {
-            const uint32_t a0 = widen(r[2 * x]), a1 = widen(r[2 * x + 1]);
-            const uint32_t a2 = widen(r[2 * x] >> 16), a3 = widen(r[2 * x + 1] >> 16);
+            uint32_t a0, a1, a2, a3;
+            widen4(r[2 * x], a0, a2);
+            widen4(r[2 * x + 1], a1, a3);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-              mma_f16(s[nt][MT == 2 ? u : x], a0, a1, a2, a3, qf[nt][k + x][0], qf[nt][k + x][1]);
+              mma_f16(s[nt][MT == 2 ? 2 * u + x : (k + x) & 3], a0, a1, a2, a3, qf[nt][k + x][0],
+                      qf[nt][k + x][1]);
           }
         }
       }
     }
-    uint32_t ph[NT][MT][2], pl[NT][MT][2];
+    uint32_t ph[NT][MT][2], pl[NT][MT][2];  // P transposed: bf16 and its remainder, or fp16
     bool moved = false;
     float keep[NT][2];
 #pragma unroll
@@ -653,7 +627,9 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
       for (int u = 0; u < MT; ++u) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          x[u][j] = (MT == 2 ? s[nt][u][j] : s[nt][0][j] + s[nt][1][j]) * fac[nt][j & 1];
+          x[u][j] = (MT == 2 ? s[nt][2 * u][j] + s[nt][2 * u + 1][j]
+                             : (s[nt][0][j] + s[nt][1][j]) + (s[nt][2][j] + s[nt][3][j])) *
+                    fac[nt][j & 1];
         const int rows = rows_of >> (8 * u) & 255;
         if (rows < kSub) {
           if (g >= rows) x[u][0] = x[u][1] = -INFINITY;
@@ -706,36 +682,44 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
 #pragma unroll
           for (int j = 0; j < 4; ++j) o[nt][k][j] *= keep[nt][j & 1];
     }
+    const uint32_t vt = at0 + kSub * S::kPitch;
+    if constexpr (!kE4m3) {
 #pragma unroll
-    for (int u = 0; u < MT; ++u) {
-      const uint32_t vt = at0 + u * S::kSubBytes + kSub * S::kPitch;
-      if constexpr (!kE4m3) {
-        const uint32_t at =
-            vt + ((lane & 7) + ((lane >> 4) << 3)) * S::kPitch + ((lane >> 3) & 1) * 16;
+      for (int u = 0; u < MT; ++u) {
+        const uint32_t at = vt + u * S::kSubBytes +
+                            S::piece((lane & 7) + ((lane >> 4) << 3), (lane >> 3) & 1);
 #pragma unroll
-        for (int k = 0; k < kBlocks; ++k) {
-          uint32_t r[4];
-          ldsm4t(r, at + k * 32);
+        for (int k0 = 0; k0 < kBlocks; k0 += 4) {
+          uint32_t r[4][4];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            mma16816(o[nt][k], r[0], r[1], r[2], r[3], ph[nt][u][0], ph[nt][u][1]);
-            mma16816(o[nt][k], r[0], r[1], r[2], r[3], pl[nt][u][0], pl[nt][u][1]);
-          }
+          for (int k = 0; k < 4 && k0 + k < kBlocks; ++k) ldsm4t(r[k], S::along(at, (k0 + k) * 32));
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int k = 0; k < 4 && k0 + k < kBlocks; ++k)
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                const uint32_t (&p)[2] = y == 0 ? ph[nt][u] : pl[nt][u];
+                mma_bf16(o[nt][k0 + k], r[k], p[0], p[1]);
+              }
         }
-      } else {
-        const uint32_t at = vt + ((lane & 7) + (lane & 8)) * S::kPitch + (lane >> 4) * 16;
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < MT; ++u) {
+        const uint32_t at =
+            vt + u * S::kSubBytes + S::piece((lane & 7) + (lane & 8), lane >> 4);
 #pragma unroll
         for (int k = 0; k < kBlocks; k += 2) {
           uint32_t r[4];
-          if (k + 1 < kBlocks) ldsm4t(r, at + k * 16);
-          else ldsm2t(r[0], r[1], at + k * 16);
+          if (k + 1 < kBlocks) ldsm4t(r, S::along(at, k * 16));
+          else ldsm2t(r[0], r[1], S::along(at, k * 16));
 #pragma unroll
           for (int x = 0; x < 2 && k + x < kBlocks; ++x) {
-            // bytes: token 2c dims 2g, 2g + 1, token 2c + 1 the same; paired by dim
-            const uint32_t lo = __byte_perm(r[2 * x], 0, 0x3120);
-            const uint32_t hi = __byte_perm(r[2 * x + 1], 0, 0x3120);
-            const uint32_t a0 = widen(lo), a1 = widen(lo >> 16);
-            const uint32_t a2 = widen(hi), a3 = widen(hi >> 16);
+            // bytes: token 2c dims 2g, 2g + 1, token 2c + 1 the same
+            uint32_t a0, a1, a2, a3;
+            widen4(r[2 * x], a0, a1);
+            widen4(r[2 * x + 1], a2, a3);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
               mma_f16(o[nt][k + x], a0, a1, a2, a3, ph[nt][u][0], ph[nt][u][1]);
@@ -769,47 +753,35 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
     }
   };
 
-  auto split_of = [&](int seg_end) {
-    const int last = cut.run_of(seg_end - 1);
-    return Split{sb, shc, last, cut.begin(last + 1) > seg_end};
-  };
-
-  // ---- the run, or runs
+  // ---- the run
   int tail = 0;  // 1: a partial segment is left in registers, 2: it has the first tile, 4: the last
-  int pos = 0;   // line position
   Split split{-1, 0, 0, 0};
   if (worker < workers) {
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) load(i);
+    for (int i = 0; i < kStages; ++i) load(i);
     // the first segment's q comes while the first tiles do
     bool open = true, from_start = start.z == 0;
     begin_segment(start.x, start.y);
-    int stage = 0, free_stage = kStages - 1, run = worker;
+    int stage = 0, pos = line.begin(worker);  // place on the line
     while (true) {
-      cp_wait<kStages - 2>();
+      cp_wait<kStages - 1>();
       __syncwarp();
-      load(free_stage);
       const int4 info = s_info[warp][stage];
       if (info.x < 0) break;
-      if (info.z & kRunFirst) {
-        if constexpr (kClaim) run = s_run[warp][stage];
-        pos = cut.begin(run);
-      }
       if (!open) {
-        open = true;
-        from_start = info.z & kSegFirst;
+        open = from_start = true;
         begin_segment(info.x, info.y);
       }
       ++pos;
       if (info.z & 0xffff) tile(stage, info.z);
-      free_stage = stage;
+      __syncwarp();
+      load(stage);  // at once: no stage is empty while the warp waits for the next
       stage = stage + 1 == kStages ? 0 : stage + 1;
       const bool done = info.w == 1, run_ends = info.z & kRunLast;
       if (done || run_ends) {
         sum_l();
         open = false;
-        const bool whole = done && from_start;
-        if (whole) {
+        if (done && from_start) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             const float i0 = R::inverse(a, shc, l[nt][0]), i1 = R::inverse(a, shc, l[nt][1]);
@@ -820,16 +792,13 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
                        lane);
             R::store_lse(a, sb, shc, nt, m[nt][0], l[nt][0], m[nt][1], l[nt][1], lane);
           }
-        } else if (kClaim || !run_ends) {
-          store_slot(a.ws.slot(run, run_ends ? 0 : 1, S::kSlot));
+        } else if (!run_ends) {
+          store_slot(a.ws.slot(worker, 1, S::kSlot));
         } else {
           tail = 1 | (from_start ? 2 : 0) | (done ? 4 : 0);
-        }
-        if (run_ends) {
-          if (from_start && !done) split = split_of(pos + info.w - 1);
-          if constexpr (kClaim) {
-            if (lane == 0) a.ws.splits()[run] = split;
-            split.b = -1;
+          if (from_start) {
+            const int seg_end = pos + info.w - 1, last = line.run_of(seg_end - 1);
+            split = Split{sb, shc, last, line.begin(last + 1) > seg_end};
           }
         }
       }
@@ -838,7 +807,6 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
     __syncwarp();
     if (tail) store_slot(reinterpret_cast<float*>(ring));
   }
-  if constexpr (kClaim) return;
   if (lane == 0) {
     s_tail[warp] = make_int4(tail, sb, shc, 0);
     s_split[warp] = split;
@@ -923,19 +891,20 @@ struct Joined {
   }
 };
 
-constexpr int kJoinWarps = 4, kJoinBatch = 8, kJoinY = 8;
+constexpr int kJoinWarps = 4, kJoinBatch = 4, kJoinY = 8;
 
-// Joins the partial results of the segments that cross runs. CTA (x, y) takes the splits
-// left by runs x * kWarps on (those of CTA x of the main kernel, where runs are not
-// claimed), output blocks y, y + gridDim.y, ... A split between two neighbours has two
-// parts: one warp each. A longer one (up to every run, for one long request) has its parts
-// dealt to the four warps, each loading eight at a time, and joined in shared memory: the
-// joining of 19 parts waits for memory twice, not 19 times.
-template <int D, bool kE4m3, int NT, bool kClaim>
+// Joins the partial results of the segments that cross runs. The splits left by runs
+// the warps of the main kernel's CTA x belong to
+// CTAs (x, 0 .. gridDim.y - 1). A split between two neighbours has two parts: one warp of
+// CTA (x, 0) each, loading four output blocks of both at once. A longer one (up to every
+// run, for one long request) is shared by the CTAs, output blocks y, y + gridDim.y, ...;
+// its parts are dealt to the four warps, each loading four at a time, and joined in shared
+// memory: the joining of 19 parts waits for memory twice, not 19 times.
+template <int D, bool kE4m3, int NT>
 __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(PagedArgs a) {
   using S = Shape<D, kE4m3, NT>;
   using R = Rows<D, kE4m3, NT>;
-  constexpr int kWarps = S::kWarps;
+  constexpr int kWarps = S::kWarps, kAll = NT * S::kBlocks;
   __shared__ float4 s_acc[kJoinWarps][32];
   __shared__ float4 s_ml[kJoinWarps][32];
   allow_dependent_launch();
@@ -943,37 +912,51 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(PagedArgs a
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane & 3;
   const int first = blockIdx.x * kWarps;
   int4 mine = make_int4(-1, 0, 0, 0);
-  if (lane < kWarps && (!kClaim || first + lane < a.ws.header()->runs))
-    mine = reinterpret_cast<const int4*>(a.ws.splits())[first + lane];
-  // parts between the first run's and the last one's: of every run, or (joined already in
-  // the CTA) of every further CTA
-  const int mid_mine = kClaim ? mine.z - mine.w - (first + lane)
-                              : (mine.z - mine.w) / kWarps - static_cast<int>(blockIdx.x);
+  if (lane < kWarps) mine = reinterpret_cast<const int4*>(a.ws.splits())[first + lane];
+  // parts between the first run's and the last one's: one of every further CTA
+  const int mid_mine = (mine.z - mine.w) / kWarps - static_cast<int>(blockIdx.x);
   const unsigned near = __ballot_sync(0xffffffffu, mine.x >= 0 && mid_mine == 0);
   unsigned far = __ballot_sync(0xffffffffu, mine.x >= 0 && mid_mine > 0);
 
-  auto add = [&](Joined& j, const float* p, int nt, int at) {
-    const float2 m = *reinterpret_cast<const float2*>(p + S::kOut + nt * 8 + 2 * c);
-    const float2 l = *reinterpret_cast<const float2*>(p + S::kOut + NT * 8 + nt * 8 + 2 * c);
-    j.add(m.x, m.y, l.x, l.y, reinterpret_cast<const float4*>(p)[at * 32 + lane]);
+  auto top_of = [&](const float* p, int nt) {
+    return *reinterpret_cast<const float2*>(p + S::kOut + nt * 8 + 2 * c);
+  };
+  auto sum_of = [&](const float* p, int nt) {
+    return *reinterpret_cast<const float2*>(p + S::kOut + NT * 8 + nt * 8 + 2 * c);
   };
   auto finish = [&](const Joined& j, int b, int hc, int nt, int k) {
     R::store(a, b, hc, nt, k, j.acc, R::inverse(a, hc, j.sum0), R::inverse(a, hc, j.sum1), lane);
     if (k == 0) R::store_lse(a, b, hc, nt, j.top0, j.sum0, j.top1, j.sum1, lane);
   };
 
-  unsigned left = near;
+  unsigned left = blockIdx.y == 0 ? near : 0;
   for (int turn = 0; left; ++turn, left &= left - 1) {
     const int i = __ffs(left) - 1;
     const int b = __shfl_sync(0xffffffffu, mine.x, i), hc = __shfl_sync(0xffffffffu, mine.y, i);
     const int last = __shfl_sync(0xffffffffu, mine.z, i);
     if (turn % kJoinWarps != warp) continue;
-    for (int at = blockIdx.y; at < NT * S::kBlocks; at += gridDim.y) {
-      const int nt = at / S::kBlocks;
-      Joined j;
-      add(j, a.ws.slot(first + i, 0, S::kSlot), nt, at);
-      add(j, a.ws.slot(last, 1, S::kSlot), nt, at);
-      finish(j, b, hc, nt, at % S::kBlocks);
+    const float *p = a.ws.slot(first + i, 0, S::kSlot), *q = a.ws.slot(last, 1, S::kSlot);
+#pragma unroll 1
+    for (int nt = 0; nt < NT; ++nt) {
+      const float2 pm = top_of(p, nt), pl = sum_of(p, nt), qm = top_of(q, nt), ql = sum_of(q, nt);
+#pragma unroll 1
+      for (int k0 = 0; k0 < S::kBlocks; k0 += kJoinBatch) {
+        float4 x[kJoinBatch], y[kJoinBatch];
+#pragma unroll
+        for (int u = 0; u < kJoinBatch; ++u) {
+          const int at = (nt * S::kBlocks + min(k0 + u, S::kBlocks - 1)) * 32 + lane;
+          x[u] = reinterpret_cast<const float4*>(p)[at];
+          y[u] = reinterpret_cast<const float4*>(q)[at];
+        }
+#pragma unroll
+        for (int u = 0; u < kJoinBatch; ++u) {
+          if (k0 + u >= S::kBlocks) break;
+          Joined j;
+          j.add(pm.x, pm.y, pl.x, pl.y, x[u]);
+          j.add(qm.x, qm.y, ql.x, ql.y, y[u]);
+          finish(j, b, hc, nt, k0 + u);
+        }
+      }
     }
   }
   for (; far; far &= far - 1) {
@@ -984,21 +967,23 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(PagedArgs a
     const int mid = __shfl_sync(0xffffffffu, mid_mine, i);
     const int parts = 1 + mid + head;
     auto part = [&](int x) -> const float* {  // in line order
-      const int run = x == 0 ? first + i : x > mid ? last
-                      : kClaim ? first + i + x : (static_cast<int>(blockIdx.x) + x) * kWarps;
+      const int run = x == 0 ? first + i
+                      : x > mid ? last : (static_cast<int>(blockIdx.x) + x) * kWarps;
       return a.ws.slot(run, x > mid ? 1 : 0, S::kSlot);
     };
-    for (int at = blockIdx.y; at < NT * S::kBlocks; at += gridDim.y) {
+#pragma unroll 1
+    for (int at = blockIdx.y; at < kAll; at += gridDim.y) {
       const int nt = at / S::kBlocks;
       Joined j;
+#pragma unroll 1
       for (int x0 = warp; x0 < parts; x0 += kJoinWarps * kJoinBatch) {
         float2 m[kJoinBatch], l[kJoinBatch];
         float4 v[kJoinBatch];
 #pragma unroll
         for (int u = 0; u < kJoinBatch; ++u) {  // all loads first; absent parts are left out
           const float* p = part(min(x0 + u * kJoinWarps, parts - 1));
-          m[u] = *reinterpret_cast<const float2*>(p + S::kOut + nt * 8 + 2 * c);
-          l[u] = *reinterpret_cast<const float2*>(p + S::kOut + NT * 8 + nt * 8 + 2 * c);
+          m[u] = top_of(p, nt);
+          l[u] = sum_of(p, nt);
           v[u] = reinterpret_cast<const float4*>(p)[at * 32 + lane];
         }
 #pragma unroll
@@ -1026,58 +1011,32 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(PagedArgs a
 // registers).
 int heads_per_segment(int group, int head_dim) { return group > 8 && head_dim <= 128 ? 16 : 8; }
 
-// How a call is spread, from its sizes and the longest lengths that its table allows.
-struct Spread {
-  int64_t ctas;  // one per SM, fewer where the longest possible line is shorter
-  int64_t runs;  // runs that the workspace has room for
-  bool claim;    // runs are claimed as warps come free (see Cut)
-};
-Spread spread_of(int64_t batch, int hkv, int group, int head_dim, bool e4m3, int64_t max_len) {
-  const int row = head_dim * (e4m3 ? 1 : 2), tile = row <= 192 ? 2 * kSub : kSub;
-  const int warps = head_dim == 256 && !e4m3 ? 4 : 8;
-  const int per = heads_per_segment(group, head_dim);
+// CTAs of the main kernel: one per SM, fewer where the longest line that the table allows is
+// shorter.
+int64_t ctas_of(int64_t batch, int hkv, int group, int head_dim, bool e4m3, int64_t max_len) {
+  const int tile = subtiles(head_dim, e4m3) * kSub, per = heads_per_segment(group, head_dim);
+  const int warps = warps_per_cta(head_dim, e4m3, per);
   const int64_t tiles = (max_len + tile - 1) / tile * batch * hkv * ((group + per - 1) / per);
-  Spread s;
-  s.ctas = std::max<int64_t>(
-      1, std::min<int64_t>(std::min<int64_t>(sm_count(), kMaxWorkers / warps),
-                           (tiles + warps - 1) / warps));
-  const int64_t workers = s.ctas * warps;
-  s.claim = tiles >= workers * kLeastClaimed && batch <= kCutBatch;
-  s.runs = s.claim ? workers * (1 + kSmall) : workers;
-  return s;
+  return std::max<int64_t>(1, std::min<int64_t>(sm_count(), (tiles + warps - 1) / warps));
 }
 
 template <int D, bool kE4m3, int NT>
 void launch(PagedArgs a, cudaStream_t st) {
   using S = Shape<D, kE4m3, NT>;
   a.chunks = (a.group + 8 * NT - 1) / (8 * NT);
-  const Spread sp = spread_of(a.batch, a.hkv, a.group, D, kE4m3, a.max_len);
-  a.ws.runs = sp.runs;
+  const unsigned ctas =
+      static_cast<unsigned>(ctas_of(a.batch, a.hkv, a.group, D, kE4m3, a.max_len));
+  a.ws.runs = static_cast<int64_t>(ctas) * S::kWarps;
   static std::once_flag once[64];
   int dev = 0;
   cudaGetDevice(&dev);
   std::call_once(once[dev & 63], [] {
-    constexpr int smem = static_cast<int>(S::kSmem);
-    cudaFuncSetAttribute(paged_attn_kernel<D, kE4m3, NT, false>,
-                         cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    cudaFuncSetAttribute(paged_attn_kernel<D, kE4m3, NT, true>,
-                         cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaFuncSetAttribute(paged_attn_kernel<D, kE4m3, NT>,
+                         cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::kSmem));
   });
-  prefer_max_shared<paged_join_kernel<D, kE4m3, NT, false>>();
-  prefer_max_shared<paged_join_kernel<D, kE4m3, NT, true>>();
-  prefer_max_shared<paged_cut_kernel>();
-  const unsigned ctas = static_cast<unsigned>(sp.ctas);
-  const dim3 threads(S::kWarps * 32), joins(static_cast<unsigned>(sp.runs / S::kWarps),
-                                            std::min(kJoinY, NT * S::kBlocks));
-  if (sp.claim) {
-    launch_pdl(paged_cut_kernel, dim3(kCutCtas), dim3(kCutThreads), a.batch * sizeof(int), st, a,
-               D, S::kTile, static_cast<int>(ctas) * S::kWarps);
-    launch_pdl(paged_attn_kernel<D, kE4m3, NT, true>, dim3(ctas), threads, S::kSmem, st, a);
-    launch_pdl(paged_join_kernel<D, kE4m3, NT, true>, joins, dim3(kJoinWarps * 32), 0, st, a);
-  } else {
-    launch_pdl(paged_attn_kernel<D, kE4m3, NT, false>, dim3(ctas), threads, S::kSmem, st, a);
-    launch_pdl(paged_join_kernel<D, kE4m3, NT, false>, joins, dim3(kJoinWarps * 32), 0, st, a);
-  }
+  prefer_max_shared<paged_join_kernel<D, kE4m3, NT>>();
+  launch_pdl(paged_attn_kernel<D, kE4m3, NT>, dim3(ctas), dim3(S::kWarps * 32), S::kSmem, st, a);
+  launch_pdl(paged_join_kernel<D, kE4m3, NT>, dim3(ctas, kJoinY), dim3(kJoinWarps * 32), 0, st, a);
 }
 
 template <int D>
@@ -1104,9 +1063,11 @@ extern "C" size_t umic_paged_attention_workspace_bytes(int64_t batch, int32_t hq
   if (batch <= 0 || hq <= 0 || hkv <= 0 || head_dim <= 0 || max_pages < 0 || page_size <= 0 ||
       hq / hkv == 0)
     return 0;
-  const Spread s = spread_of(batch, hkv, hq / hkv, head_dim, cache_dtype == UMIC_DTYPE_E4M3,
-                             max_pages * page_size);
-  return Space::bytes(s.runs, heads_per_segment(hq / hkv, head_dim) * (head_dim + 2));
+  const bool e4m3 = cache_dtype == UMIC_DTYPE_E4M3;
+  const int per = heads_per_segment(hq / hkv, head_dim);
+  return Space::bytes(ctas_of(batch, hkv, hq / hkv, head_dim, e4m3, max_pages * page_size) *
+                          warps_per_cta(head_dim, e4m3, per),
+                      per * (head_dim + 2));
 }
 
 extern "C" int umic_paged_attention(
@@ -1175,6 +1136,7 @@ extern "C" int umic_paged_attention(
   a.pg_sp = pg_sp * es; a.pg_sh = pg_sh * es; a.pg_ss = pg_ss * es;
   a.table_stride = table_stride;
   a.max_len = static_cast<int32_t>(max_pages * page_size);
+  a.max_pages = static_cast<int32_t>(max_pages);
   a.num_pages = num_pages;
   a.page_size = static_cast<int32_t>(page_size);
   a.hq = hq; a.hkv = hkv; a.batch = static_cast<int32_t>(batch); a.group = hq / hkv;

@@ -19,7 +19,7 @@ from typing import NamedTuple
 import torch
 
 from .. import _lib
-from ._common import require_bf16, require_cuda, stats
+from ._common import require_cuda, stats
 from .rmsnorm import _w_dtype
 
 E4M3 = torch.float8_e4m3fn
@@ -36,13 +36,37 @@ class PagedPlan(NamedTuple):
     positions: torch.Tensor
 
 
-def _require(name: str, what: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple) -> None:
-    if t.dtype != dtype:
+# The checks below are most of what a small call costs on the host: each reads a tensor's
+# shape, strides, dtype and device once.
+
+def _one_device(name: str, first: torch.Tensor, *rest: torch.Tensor | None) -> torch.device:
+    dev = first.device
+    for t in rest:
+        if t is not None and t.device != dev:
+            require_cuda(name, first, *rest)
+    if not first.is_cuda:
+        require_cuda(name, first)
+    return dev
+
+
+def _require(name: str, what: str, t: torch.Tensor, dtype: torch.dtype, *shape: int) -> None:
+    if t.dtype is not dtype:
         raise TypeError(f"{name}: {what} must be {dtype}, got {t.dtype}")
     if t.shape != shape:
         raise ValueError(f"{name}: {what} {tuple(t.shape)}, expected {shape}")
     if not t.is_contiguous():
         raise ValueError(f"{name}: {what} must be contiguous")
+
+
+def _table(name: str, table: torch.Tensor, n: int) -> tuple[int, int]:
+    """Row stride and width of a block table of n rows."""
+    if table.dtype is torch.int32 and table.ndim == 2:
+        rows, width = table.shape
+        stride, unit = table.stride()
+        if rows == n and (unit == 1 or width <= 1):
+            return stride, width
+    raise ValueError(f"{name}: block_table must be int32 [{n}, max_pages] with its rows "
+                     f"contiguous, got {table.dtype} {tuple(table.shape)}")
 
 
 def paged_plan(kv_lens: torch.Tensor, new_tokens: torch.Tensor, block_table: torch.Tensor,
@@ -59,136 +83,135 @@ def paged_plan(kv_lens: torch.Tensor, new_tokens: torch.Tensor, block_table: tor
     not keeps what it had, gets slots of -1 and sets DEVERR_PAGES (umic_b200.device_errors).
     out_lens may be kv_lens and out_span may be free_span (then they advance in place).
     """
-    dev = require_cuda("paged_plan", kv_lens, new_tokens, block_table, free_ring, free_span,
-                       out_lens, out_span)
-    n = kv_lens.shape[0] if kv_lens.dim() == 1 else -1
-    _require("paged_plan", "kv_lens", kv_lens, torch.int32, (n,))
-    _require("paged_plan", "new_tokens", new_tokens, torch.int32, (n,))
-    _require("paged_plan", "free_span", free_span, torch.int64, (2,))
-    pages = free_ring.numel()
-    _require("paged_plan", "free_ring", free_ring, torch.int32, (pages,))
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != n \
-            or (block_table.stride(1) != 1 and block_table.shape[1] > 1):
-        raise ValueError(f"paged_plan: block_table must be int32 [{n}, max_pages] with its rows "
-                         f"contiguous, got {block_table.dtype} {tuple(block_table.shape)}")
+    dev = _one_device("paged_plan", kv_lens, new_tokens, block_table, free_ring, free_span,
+                      out_lens, out_span)
+    n, pages = kv_lens.numel(), free_ring.numel()
+    _require("paged_plan", "kv_lens", kv_lens, torch.int32, n)
+    _require("paged_plan", "new_tokens", new_tokens, torch.int32, n)
+    _require("paged_plan", "free_span", free_span, torch.int64, 2)
+    _require("paged_plan", "free_ring", free_ring, torch.int32, pages)
+    stride, width = _table("paged_plan", block_table, n)
     capacity = int(capacity)
     if capacity < 0:
         raise ValueError(f"paged_plan: capacity {capacity}")
-    # one allocation: span (2 x int64), token offsets, lengths, slots, positions
-    buf = torch.empty(5 + 2 * n + 2 * capacity, dtype=torch.int32, device=dev)
-    span, cu, lens, slots, positions = buf.split((4, n + 1, n, capacity, capacity))
     if out_lens is None:
-        out_lens = lens
+        out_lens = torch.empty_like(kv_lens)
     else:
-        _require("paged_plan", "out_lens", out_lens, torch.int32, (n,))
+        _require("paged_plan", "out_lens", out_lens, torch.int32, n)
     if out_span is None:
-        out_span = span.view(torch.int64)
+        out_span = torch.empty_like(free_span)
     else:
-        _require("paged_plan", "out_span", out_span, torch.int64, (2,))
+        _require("paged_plan", "out_span", out_span, torch.int64, 2)
+    cu, slots = kv_lens.new_empty(n + 1), kv_lens.new_empty(capacity)
+    positions = kv_lens.new_empty(capacity)
     _lib.call("umic_paged_plan", dev, kv_lens.data_ptr(), new_tokens.data_ptr(), n,
-              block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
-              free_ring.data_ptr(), pages, free_span.data_ptr(), int(page_size),
-              out_lens.data_ptr(), out_span.data_ptr(), cu.data_ptr(), slots.data_ptr(),
-              positions.data_ptr(), capacity)
+              block_table.data_ptr(), stride, width, free_ring.data_ptr(), pages,
+              free_span.data_ptr(), page_size, out_lens.data_ptr(), out_span.data_ptr(),
+              cu.data_ptr(), slots.data_ptr(), positions.data_ptr(), capacity)
     stats["umic_paged_plan"] += 1
     return PagedPlan(out_lens, out_span, cu, slots, positions)
 
 
 def _check_pages(name: str, k_pages: torch.Tensor, v_pages: torch.Tensor,
-                 k_scale: torch.Tensor | None, v_scale: torch.Tensor | None) -> int:
-    """Checks a pool and its scales; returns its dtype code."""
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or \
-            k_pages.stride() != v_pages.stride() or k_pages.dtype != v_pages.dtype:
+                 k_scale: torch.Tensor | None, v_scale: torch.Tensor | None) -> tuple:
+    """Checks a pool and its scales; returns its dtype code, shape and strides."""
+    shape, strides, dtype = k_pages.shape, k_pages.stride(), k_pages.dtype
+    if len(shape) != 4 or shape != v_pages.shape or strides != v_pages.stride() or \
+            dtype is not v_pages.dtype:
         raise ValueError(f"{name}: k_pages and v_pages must be [num_pages, kv_heads, page_size, "
                          "head_dim] of one shape, strides and dtype")
-    if k_pages.stride(3) != 1:
+    if strides[3] != 1:
         raise ValueError(f"{name}: head_dim must be contiguous in the pages")
-    if k_pages.dtype == torch.bfloat16:
+    if dtype is torch.bfloat16:
         if k_scale is not None or v_scale is not None:
             raise ValueError(f"{name}: scales belong to {E4M3} pages")
-        return _lib.DTYPE_BF16
-    if k_pages.dtype != E4M3:
-        raise TypeError(f"{name}: pages must be bfloat16 or {E4M3}, got {k_pages.dtype}")
-    for what, s in (("k_scale", k_scale), ("v_scale", v_scale)):
-        if s is not None:
-            _require(name, what, s, torch.float32, (k_pages.shape[1],))
-    return _lib.DTYPE_E4M3
+        return _lib.DTYPE_BF16, shape, strides
+    if dtype is not E4M3:
+        raise TypeError(f"{name}: pages must be bfloat16 or {E4M3}, got {dtype}")
+    if k_scale is not None:
+        _require(name, "k_scale", k_scale, torch.float32, shape[1])
+    if v_scale is not None:
+        _require(name, "v_scale", v_scale, torch.float32, shape[1])
+    return _lib.DTYPE_E4M3, shape, strides
+
+
+def _rows(name: str, what: str, x: torch.Tensor, t: int, heads: int | None, d: int) -> tuple:
+    """(pointer, token stride, head stride, heads) of [t, heads, d] bf16 rows."""
+    if x.dtype is not torch.bfloat16:
+        raise TypeError(f"{name}: {what} must be bfloat16, got {x.dtype}")
+    shape, strides = x.shape, x.stride()
+    if len(shape) != 3 or shape[0] != t or shape[2] != d or strides[2] != 1 or \
+            (heads is not None and shape[1] != heads):
+        raise ValueError(f"{name}: {what} {tuple(shape)} / strides {strides}, expected "
+                         f"[{t}, {'heads' if heads is None else heads}, {d}] with head_dim "
+                         "contiguous")
+    return x.data_ptr(), strides[0], strides[1], shape[1]
 
 
 def _input(name, q, k, v, positions, inv_freq, sections, interleaved, scaling, q_weight,
            k_weight, q_eps, k_eps, k_pages, v_pages, slots, k_scale, v_scale, q_out, k_out):
-    dev = require_cuda(name, q, k, v, positions, inv_freq, q_weight, k_weight, k_pages, v_pages,
-                       slots, k_scale, v_scale, q_out, k_out)
-    require_bf16(name, q, k, v, q_out, k_out)
-    if k.dim() != 3:
+    dev = _one_device(name, k, q, v, positions, inv_freq, q_weight, k_weight, k_pages, v_pages,
+                      slots, k_scale, v_scale, q_out, k_out)
+    if k.ndim != 3:
         raise ValueError(f"{name}: k must be [tokens, heads, head_dim], got {tuple(k.shape)}")
     t, hk, d = k.shape
-    for what, x in (("q", q), ("k", k), ("v", v), ("q_out", q_out), ("k_out", k_out)):
-        if x is None:
-            continue
-        if x.dim() != 3 or x.shape[0] != t or x.shape[2] != d or x.stride(2) != 1 or \
-                (what not in ("q", "q_out") and x.shape[1] != hk):
-            raise ValueError(f"{name}: {what} {tuple(x.shape)} / strides {x.stride()} does not "
-                             f"match k {tuple(k.shape)} (head_dim contiguous)")
-    if q_out is not None and q_out.shape != q.shape:
-        raise ValueError(f"{name}: q_out {tuple(q_out.shape)} for q {tuple(q.shape)}")
+    ka = _rows(name, "k", k, t, hk, d)
+    va = (None, 0, 0) if v is None else _rows(name, "v", v, t, hk, d)[:3]
     if k_pages is None:
         if v_pages is not None or slots is not None or k_scale is not None or \
                 v_scale is not None:
             raise ValueError(f"{name}: v_pages, slots and scales go with k_pages")
-        pool, dt, slots_ptr = (0, 0, 0, 0, 0), _lib.DTYPE_BF16, None
+        if k_out is None:
+            k_out = k.new_empty((t, hk, d))
+        ko = _rows(name, "k_out", k_out, t, hk, d)[:3]
+        pool = (None, None, 0, 0, 0, 0, 0, _lib.DTYPE_BF16, None, None, None)
     else:
         if v is None or v_pages is None or slots is None:
             raise ValueError(f"{name}: a cache write needs v, v_pages and slots")
-        dt = _check_pages(name, k_pages, v_pages, k_scale, v_scale)
-        if k_pages.shape[1] != hk or k_pages.shape[3] != d:
-            raise ValueError(f"{name}: pages {tuple(k_pages.shape)} do not match k "
-                             f"{tuple(k.shape)}")
-        _require(name, "slots", slots, torch.int32, (t,))
-        pool = (*k_pages.stride()[:3], k_pages.shape[0], k_pages.shape[2])
-        slots_ptr = slots.data_ptr()
-    w = q_weight if q_weight is not None else k_weight
-    if w is not None:
-        for what, x in (("q_weight", q_weight), ("k_weight", k_weight)):
-            if x is not None:
-                _require(name, what, x, w.dtype, (d,))
+        if k_out is not None:
+            raise ValueError(f"{name}: k_out goes without k_pages")
+        dt, shape, strides = _check_pages(name, k_pages, v_pages, k_scale, v_scale)
+        if shape[1] != hk or shape[3] != d:
+            raise ValueError(f"{name}: pages {tuple(shape)} do not match k {tuple(k.shape)}")
+        _require(name, "slots", slots, torch.int32, t)
+        pool = (k_pages.data_ptr(), v_pages.data_ptr(), strides[0], strides[1], strides[2],
+                shape[0], shape[2], dt, _lib.ptr(k_scale), _lib.ptr(v_scale), slots.data_ptr())
+        ko = (None, 0, 0)
+    if q is None:
+        qa, qo = (None, 0, 0, 0), (None, 0, 0)
+    else:
+        qa = _rows(name, "q", q, t, None, d)
+        if q_out is None:
+            q_out = q.new_empty((t, qa[3], d))
+        qo = _rows(name, "q_out", q_out, t, qa[3], d)[:3]
+    wdt = _lib.DTYPE_BF16
+    if q_weight is not None or k_weight is not None:
+        w = q_weight if q_weight is not None else k_weight
+        wdt = _w_dtype(w)
+        _require(name, "q_weight", w, w.dtype, d)
+        if k_weight is not None:
+            _require(name, "k_weight", k_weight, w.dtype, d)
     if positions is None:
         rot = (None, 4, 0, 0, None, 0, 1, 0, 0, 0, 0)
     else:
-        if positions.dim() == 1:
-            positions = positions[None]
-        axes = positions.shape[0]
-        if positions.dtype not in (torch.int32, torch.int64) or positions.dim() != 2 or \
-                positions.shape[1] != t or not 1 <= axes <= 3 or len(sections) != axes:
+        axes, (p_sa, p_st) = 1, (0, 1)
+        if positions.ndim == 2:
+            axes, (p_sa, p_st) = positions.shape[0], positions.stride()
+        elif positions.ndim == 1:
+            p_st = positions.stride(0)
+        if positions.dtype not in (torch.int32, torch.int64) or positions.ndim not in (1, 2) or \
+                positions.shape[-1] != t or not 1 <= axes <= 3 or len(sections) != axes:
             raise ValueError(f"{name}: positions must be int32 or int64 [axes, {t}] with one of "
                              f"{len(sections)} sections per axis (1 to 3), got "
                              f"{positions.dtype} {tuple(positions.shape)}")
         half = inv_freq.numel()
-        _require(name, "inv_freq", inv_freq, torch.float32, (half,))
-        sec = (*map(int, sections), 0, 0)
-        rot = (positions.data_ptr(), positions.element_size(),
-               positions.stride(0), positions.stride(1), inv_freq.data_ptr(),
-               2 * half, axes, sec[0], sec[1], sec[2], int(interleaved))
-    if q is None:
-        qa, qo = (None, 0, 0, 0), (None, 0, 0)
-    else:
-        if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        qa = (q.data_ptr(), q.stride(0), q.stride(1), q.shape[1])
-        qo = (q_out.data_ptr(), q_out.stride(0), q_out.stride(1))
-    if k_pages is None:
-        if k_out is None:
-            k_out = torch.empty(k.shape, dtype=k.dtype, device=dev)
-        ko = (k_out.data_ptr(), k_out.stride(0), k_out.stride(1))
-    else:
-        k_out, ko = None, (None, 0, 0)
-    va = (v.data_ptr(), v.stride(0), v.stride(1)) if v is not None else (None, 0, 0)
-    _lib.call("umic_qk_norm_mrope_kv", dev, *qa, k.data_ptr(), k.stride(0), k.stride(1), *va, hk,
-              *qo, *ko, _lib.ptr(q_weight), _lib.ptr(k_weight),
-              _w_dtype(w) if w is not None else _lib.DTYPE_BF16, q_eps, k_eps, *rot, scaling,
-              _lib.ptr(k_pages), _lib.ptr(v_pages), *pool, dt, _lib.ptr(k_scale),
-              _lib.ptr(v_scale), slots_ptr, t, d)
-    return q_out, k_out
+        _require(name, "inv_freq", inv_freq, torch.float32, half)
+        s0, s1, s2 = (*sections, 0, 0)[:3]
+        rot = (positions.data_ptr(), 4 if positions.dtype is torch.int32 else 8, p_sa, p_st,
+               inv_freq.data_ptr(), 2 * half, axes, s0, s1, s2, int(interleaved))
+    _lib.call("umic_qk_norm_mrope_kv", dev, *qa, *ka[:3], *va, hk, *qo, *ko, _lib.ptr(q_weight),
+              _lib.ptr(k_weight), wdt, q_eps, k_eps, *rot, scaling, *pool, t, d)
+    return q_out, (k_out if k_pages is None else None)
 
 
 def qk_norm_mrope_kv(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor | None,
@@ -245,37 +268,28 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     without tokens come out as zeros (lse -inf). D 64, 80, 96, 128 or 256; page a multiple
     of 16; any number of query heads per KV head.
     """
-    dev = require_cuda("paged_attention", q, k_pages, v_pages, block_table, kv_lens, k_scale,
-                       v_scale, out)
-    require_bf16("paged_attention", q, out)
-    dt = _check_pages("paged_attention", k_pages, v_pages, k_scale, v_scale)
-    if q.dim() != 3 or q.stride(2) != 1 or q.shape[2] != k_pages.shape[3]:
-        raise ValueError(f"paged_attention: q {tuple(q.shape)} (head_dim contiguous) for pages "
-                         f"{tuple(k_pages.shape)}")
+    dev = _one_device("paged_attention", q, k_pages, v_pages, block_table, kv_lens, k_scale,
+                      v_scale, out)
+    dt, (p, hk, page, dp), (sp, sh, ss, _) = _check_pages("paged_attention", k_pages, v_pages,
+                                                          k_scale, v_scale)
+    if q.ndim != 3 or q.shape[2] != dp:
+        raise ValueError(f"paged_attention: q {tuple(q.shape)} for pages {tuple(k_pages.shape)}")
     b, hq, d = q.shape
-    p, hk, page, _ = k_pages.shape
-    _require("paged_attention", "kv_lens", kv_lens, torch.int32, (b,))
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != b \
-            or (block_table.stride(1) != 1 and block_table.shape[1] > 1):
-        raise ValueError(f"paged_attention: block_table must be int32 [{b}, max_pages] with its "
-                         f"rows contiguous, got {block_table.dtype} "
-                         f"{tuple(block_table.shape)}")
+    qa = _rows("paged_attention", "q", q, b, hq, d)
+    _require("paged_attention", "kv_lens", kv_lens, torch.int32, b)
+    stride, width = _table("paged_attention", block_table, b)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.stride(2) != 1:
-        raise ValueError(f"paged_attention: out {tuple(out.shape)} for q {tuple(q.shape)}")
+        out = q.new_empty((b, hq, d))
+    oa = _rows("paged_attention", "out", out, b, hq, d)
     lse = torch.empty((b, hq), dtype=torch.float32, device=dev) if return_lse else None
     # its own workspace for every call: calls on several streams, and graphs captured
     # apart, never share one
     _lib._ensure_device(dev)
-    need = _lib.lib().umic_paged_attention_workspace_bytes(
-        b, hq, hk, d, block_table.shape[1], page, dt)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    _lib.call("umic_paged_attention", dev, q.data_ptr(), q.stride(0), q.stride(1),
-              k_pages.data_ptr(), v_pages.data_ptr(), *k_pages.stride()[:3], p, page, dt,
-              _lib.ptr(k_scale), _lib.ptr(v_scale), block_table.data_ptr(),
-              block_table.stride(0), block_table.shape[1], kv_lens.data_ptr(), out.data_ptr(),
-              out.stride(0), out.stride(1), _lib.ptr(lse), b, hq, hk, d, scale, ws.data_ptr(),
-              need)
+    need = _lib.lib().umic_paged_attention_workspace_bytes(b, hq, hk, d, width, page, dt)
+    ws = q.new_empty((need + 1) // 2)
+    _lib.call("umic_paged_attention", dev, qa[0], qa[1], qa[2], k_pages.data_ptr(),
+              v_pages.data_ptr(), sp, sh, ss, p, page, dt, _lib.ptr(k_scale),
+              _lib.ptr(v_scale), block_table.data_ptr(), stride, width, kv_lens.data_ptr(), oa[0],
+              oa[1], oa[2], _lib.ptr(lse), b, hq, hk, d, scale, ws.data_ptr(), need)
     stats["umic_paged_attention"] += 1
     return (out, lse) if return_lse else out
