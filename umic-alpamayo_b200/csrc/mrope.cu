@@ -8,8 +8,17 @@
 //
 // The angle is taken in 64 bits and reduced to a fraction of a turn there: in 32 bits a
 // position of 30 000 leaves 2^-9 of a radian, as much as bf16's own rounding. The rest is
-// fp32, rounded once on the way out. A warp owns one head row of one token.
+// fp32, rounded once on the way out.
+//
+// HBM bounds it: every row is read and written once. A group of TPH lanes owns a head row,
+// 16 elements a lane: 8 of the first half and their rotary partners, so the rotation needs
+// no exchange and the norm log2(TPH) shuffles. A warp takes one token and some of its row
+// groups (32 / TPH rows of q, k, v in turn), the rows of two groups loaded before either is
+// used. The token's angles are made once per warp, shared out among the row groups' lanes
+// and handed round by shuffles: 64 sines and cosines against the 24 KB of a token's 48 rows.
 #include <cuda_fp8.h>
+
+#include <algorithm>
 
 #include "common.cuh"
 
@@ -27,6 +36,7 @@ struct MropeArgs {
   int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, qo_st, qo_sh, ko_st, ko_sh;
   int64_t p_sa, p_st, pg_sp, pg_sh, pg_ss, num_slots;
   int32_t page_size, tokens, hq, hk, d, half;
+  int32_t shares, groups;  // warps of a token, row groups of each
   int32_t sec[3], axes, interleaved, pos64, w_dtype, e4m3;
   float q_eps, k_eps, scaling;
 };
@@ -45,6 +55,16 @@ __device__ __forceinline__ double position_of(const MropeArgs& a, int axis, int6
                  : static_cast<double>(static_cast<const int32_t*>(a.positions)[at]);
 }
 
+// Rows read once. Not through the read-only path: q_out may be q.
+__device__ __forceinline__ uint4 ld_row(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p)
+               : "memory");
+  return v;
+}
+
 // cos and sin of pos * freq: the product in turns, its whole part dropped, in 64 bits
 __device__ __forceinline__ void turn(double pos, float freq, float scaling, float* c, float* s) {
   const double u = pos * (static_cast<double>(freq) * 0.15915494309189533577);
@@ -53,63 +73,166 @@ __device__ __forceinline__ void turn(double pos, float freq, float scaling, floa
   *s *= scaling;
 }
 
-__device__ __forceinline__ void store_page(void* base, int64_t at, float x, bool e4m3, float scale) {
-  if (e4m3)
-    static_cast<__nv_fp8_storage_t*>(base)[at] =
-        __nv_cvt_float_to_fp8(__fdiv_rn(x, scale), __NV_SATFINITE, __NV_E4M3);
-  else
-    static_cast<__nv_bfloat16*>(base)[at] = __float2bfloat16_rn(x);
+// 8 values as e4m3 after a division by the scale (a true one: a product with the inverse
+// would fall on the other side of a border now and then).
+__device__ __forceinline__ uint2 pack8_e4m3(const float (&f)[8], float scale) {
+  uint32_t w[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 x = make_float2(__fdiv_rn(f[2 * i], scale), __fdiv_rn(f[2 * i + 1], scale));
+    w[i / 2] |= static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(x, __NV_SATFINITE, __NV_E4M3))
+                << (i % 2 * 16);
+  }
+  return make_uint2(w[0], w[1]);
 }
 
-__global__ void __launch_bounds__(128) mrope_kernel(MropeArgs a) {
+constexpr int kThreads = 256;
+constexpr int kAhead = 2;  // row groups loaded before the first is used
+
+template <int TPH, bool kE4m3>
+__global__ void __launch_bounds__(kThreads) mrope_kernel(MropeArgs a) {
   allow_dependent_launch();
   wait_prerequisite();
-  const int lane = threadIdx.x & 31;
-  const int rows = a.hq + a.hk + (a.k_pages ? a.hk : 0);
-  const int64_t task = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  const int64_t t = task / rows;
+  constexpr int kRows = 32 / TPH;     // rows of a group
+  constexpr int kShare = 8 / kRows;   // angles a lane makes (TPH >= 4, so at least one)
+  const int lane = threadIdx.x & 31, sub = lane % TPH, mine = lane / TPH;
+  const int64_t task = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+  const int t = static_cast<int>(task / a.shares);
   if (t >= a.tokens) return;
-  const int r = static_cast<int>(task % rows);
-  const bool is_q = r < a.hq, is_v = r >= a.hq + a.hk;
-  const int h = is_q ? r : is_v ? r - a.hq - a.hk : r - a.hq;
-  int64_t page_at = 0;
-  if (!is_q && a.k_pages) {
-    const int64_t slot = a.slots[t];
-    if (slot < 0 || slot >= a.num_slots) {
-      if (slot != -1 && lane == 0) atomicOr(a.err, UMIC_DEVERR_BAD_PAGE);
-      return;
-    }
-    page_at = slot / a.page_size * a.pg_sp + h * a.pg_sh + slot % a.page_size * a.pg_ss;
-  }
-  const __nv_bfloat16* x = is_q ? a.q + t * a.q_st + h * a.q_sh
-                          : is_v ? a.v + t * a.v_st + h * a.v_sh
-                                 : a.k + t * a.k_st + h * a.k_sh;
-  const void* w = is_q ? a.qw : is_v ? nullptr : a.kw;
-  float rstd = 1.f;
-  if (w) {
-    float ss = 0.f;
-    for (int i = lane; i < a.d; i += 32) ss += bf(x[i]) * bf(x[i]);
-    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    rstd = rsqrtf(ss / static_cast<float>(a.d) + (is_q ? a.q_eps : a.k_eps));
-  }
-  const float* scales = is_v ? a.v_scale : a.k_scale;
-  const float scale = !is_q && scales ? scales[h] : 1.f;
-  auto value = [&](int i) { return w ? bf(x[i]) * rstd * load_w1(w, a.w_dtype, i) : bf(x[i]); };
-  auto put = [&](int i, float y) {
-    if (is_q) a.q_out[t * a.qo_st + h * a.qo_sh + i] = __float2bfloat16_rn(y);
-    else if (!a.k_pages) a.k_out[t * a.ko_st + h * a.ko_sh + i] = __float2bfloat16_rn(y);
-    else store_page(is_v ? a.v_pages : a.k_pages, page_at + i, y, a.e4m3, scale);
+  const int rows = a.hq + a.hk + (a.k_pages ? a.hk : 0);
+  const int row0 = static_cast<int>(task % a.shares) * a.groups * kRows;
+  const int row1 = min(rows, row0 + a.groups * kRows);
+
+  const int turned = a.half / 8;  // lanes of a row whose pairs are rotated
+  const bool there = sub < a.d / 16, turns = sub < turned;
+  const int lo = turns ? sub * 8 : 2 * a.half + (sub - turned) * 16;
+  const int hi = turns ? a.half + sub * 8 : lo + 8;
+  const __nv_bfloat16* const q = a.q + t * a.q_st;
+  const __nv_bfloat16* const k = a.k + t * a.k_st;
+  const __nv_bfloat16* const v = a.v + t * a.v_st;
+  auto source = [&](int r) {
+    return r < a.hq ? q + r * a.q_sh
+           : r < a.hq + a.hk ? k + (r - a.hq) * a.k_sh : v + (r - a.hq - a.hk) * a.v_sh;
   };
-  // in-place rows: a lane reads both elements of a pair before it writes either
-  const int half = is_v ? 0 : a.half;
-  for (int i = lane; i < half; i += 32) {
-    float c, s;
-    turn(position_of(a, axis_of(a, i), t), a.inv_freq[i], a.scaling, &c, &s);
-    const float lo = value(i), hi = value(i + half);
-    put(i, lo * c - hi * s);
-    put(i + half, hi * c + lo * s);
+  uint4 xl[kAhead], xh[kAhead];
+  auto fetch = [&](int first) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int r = first + u * kRows + mine;
+      xl[u] = xh[u] = make_uint4(0, 0, 0, 0);
+      if (there && r < row1) {
+        const __nv_bfloat16* p = source(r);
+        xl[u] = ld_row(p + lo);
+        xh[u] = ld_row(p + hi);
+      }
+    }
+  };
+  fetch(row0);
+
+  int64_t page_at = -1;  // where the token's K and V go; -1: nowhere
+  if (a.k_pages && row1 > a.hq) {
+    const int slot = a.slots[t];
+    if (slot >= 0 && slot < a.num_slots) {
+      const int page = slot / a.page_size;
+      page_at = page * a.pg_sp + (slot - page * a.page_size) * a.pg_ss;
+    } else if (slot != -1 && lane == 0) {
+      atomicOr(a.err, UMIC_DEVERR_BAD_PAGE);
+    }
   }
-  for (int i = 2 * half + lane; i < a.d; i += 32) put(i, value(i));
+  float c[8], s[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    c[i] = s[i] = 0.f;
+  }
+  if (a.half && row0 < a.hq + a.hk) {
+    float mc[kShare], ms[kShare];
+#pragma unroll
+    for (int x = 0; x < kShare; ++x) {
+      const int i = min(sub * 8 + mine * kShare + x, a.half - 1);
+      turn(position_of(a, axis_of(a, i), t), a.inv_freq[i], a.scaling, &mc[x], &ms[x]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int from = i / kShare * TPH + sub;
+      const float cv = __shfl_sync(0xffffffffu, mc[i % kShare], from);
+      const float sv = __shfl_sync(0xffffffffu, ms[i % kShare], from);
+      c[i] = cv;
+      s[i] = sv;
+    }
+  }
+
+#pragma unroll 1
+  for (int first = row0; first < row1; first += kAhead * kRows) {
+    uint4 yl[kAhead], yh[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      yl[u] = xl[u];
+      yh[u] = xh[u];
+    }
+    if (first + kAhead * kRows < row1) fetch(first + kAhead * kRows);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int r = first + u * kRows + mine;
+      if (first + u * kRows >= row1) break;
+      const bool is_q = r < a.hq, is_v = r >= a.hq + a.hk;
+      const int h = is_q ? r : is_v ? r - a.hq - a.hk : r - a.hq;
+      float x[8], y[8];
+      unpack8(yl[u], x);
+      unpack8(yh[u], y);
+      if (a.qw || a.kw) {  // all lanes take part in the shuffles
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss += x[i] * x[i] + y[i] * y[i];
+#pragma unroll
+        for (int o = TPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const void* w = is_q ? a.qw : is_v ? nullptr : a.kw;
+        if (w && there) {
+          const float rstd = rsqrtf(ss / static_cast<float>(a.d) + (is_q ? a.q_eps : a.k_eps));
+          float wv[8];
+          load_w8(w, a.w_dtype, lo, wv);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = x[i] * rstd * wv[i];
+          load_w8(w, a.w_dtype, hi, wv);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) y[i] = y[i] * rstd * wv[i];
+        }
+      }
+      const bool plain = is_v || !turns;  // not "times 1 plus times 0": infinity passes
+      float ox[8], oy[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        ox[i] = plain ? x[i] : x[i] * c[i] - y[i] * s[i];
+        oy[i] = plain ? y[i] : y[i] * c[i] + x[i] * s[i];
+      }
+      if (!there || r >= row1) continue;
+      if (is_q || !a.k_pages) {
+        __nv_bfloat16* out =
+            is_q ? a.q_out + t * a.qo_st + h * a.qo_sh : a.k_out + t * a.ko_st + h * a.ko_sh;
+        st_vec(out + lo, pack8(ox));
+        st_vec(out + hi, pack8(oy));
+      } else if (page_at >= 0) {
+        const int64_t at = page_at + h * a.pg_sh;
+        if constexpr (kE4m3) {
+          const float* scales = is_v ? a.v_scale : a.k_scale;
+          const float scale = scales ? __ldg(scales + h) : 1.f;
+          uint8_t* out = static_cast<uint8_t*>(is_v ? a.v_pages : a.k_pages) + at;
+          *reinterpret_cast<uint2*>(out + lo) = pack8_e4m3(ox, scale);
+          *reinterpret_cast<uint2*>(out + hi) = pack8_e4m3(oy, scale);
+        } else {
+          __nv_bfloat16* out = static_cast<__nv_bfloat16*>(is_v ? a.v_pages : a.k_pages) + at;
+          st_vec(out + lo, pack8(ox));
+          st_vec(out + hi, pack8(oy));
+        }
+      }
+    }
+  }
+}
+
+template <int TPH>
+void launch(const MropeArgs& a, int64_t blocks, cudaStream_t st) {
+  const dim3 grid(static_cast<unsigned>(blocks));
+  if (a.e4m3) launch_pdl(mrope_kernel<TPH, true>, grid, dim3(kThreads), 0, st, a);
+  else launch_pdl(mrope_kernel<TPH, false>, grid, dim3(kThreads), 0, st, a);
 }
 
 }  // namespace
@@ -211,11 +334,20 @@ extern "C" int umic_qk_norm_mrope_kv(
   a.k_eps = k_eps;
   a.scaling = scaling;
   const int64_t rows = static_cast<int64_t>(hq) + hk + (k_pages ? hk : 0);
-  const int64_t blocks = (tokens * rows + 3) / 4;
+  const int tph = head_dim <= 64 ? 4 : head_dim <= 128 ? 8 : 16;
+  const int64_t groups = (rows + 32 / tph - 1) / (32 / tph);
+  // A warp each for a row group while that leaves the GPU's warps (64 an SM) unfilled; with
+  // more tokens longer shares, which make a token's angles fewer times.
+  const int64_t per = tokens * groups / (static_cast<int64_t>(sm_count()) * 64);
+  a.groups = static_cast<int32_t>(std::max<int64_t>(1, std::min(per, groups)));
+  a.shares = static_cast<int32_t>((groups + a.groups - 1) / a.groups);
+  const int64_t blocks = (tokens * a.shares + kThreads / 32 - 1) / (kThreads / 32);
   if (blocks > 0x7fffffffLL)
     return fail(UMIC_ERR_UNSUPPORTED, "%s: %lld tokens x %lld heads", me, (long long)tokens,
                 (long long)rows);
-  launch_pdl(mrope_kernel, dim3(static_cast<unsigned>(blocks)), dim3(128), 0, as_stream(stream),
-             a);
+  cudaStream_t st = as_stream(stream);
+  if (tph == 4) launch<4>(a, blocks, st);
+  else if (tph == 8) launch<8>(a, blocks, st);
+  else launch<16>(a, blocks, st);
   return launch_status(me);
 }
