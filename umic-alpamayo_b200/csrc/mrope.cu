@@ -10,12 +10,16 @@
 // position of 30 000 leaves 2^-9 of a radian, as much as bf16's own rounding. The rest is
 // fp32, rounded once on the way out.
 //
-// HBM bounds it: every row is read and written once. A group of TPH lanes owns a head row,
-// 16 elements a lane: 8 of the first half and their rotary partners, so the rotation needs
-// no exchange and the norm log2(TPH) shuffles. A warp takes one token and some of its row
-// groups (32 / TPH rows of q, k, v in turn), the rows of two groups loaded before either is
-// used. The token's angles are made once per warp, shared out among the row groups' lanes
-// and handed round by shuffles: 64 sines and cosines against the 24 KB of a token's 48 rows.
+// HBM bounds it: every row is read and written once, 24 KB for a token of 32 + 8 + 8 heads,
+// and the issue slots run close behind, so the work per row is kept small. A group of TPH
+// lanes owns a head row, 16 elements a lane: 8 of the first half and their rotary partners,
+// so the rotation needs no exchange and the norm log2(TPH) shuffles. A warp walks over
+// tokens and in each over row groups (32 / TPH rows of one kind: q, k or v), all of them or
+// a share; each lane copies its own pieces of the next kDepth groups, across tokens, into
+// shared memory with asynchronous loads. A token's angles are made once per warp, shared
+// out among the row groups' lanes and handed round by shuffles, times the norm's weights,
+// when the warp comes to the q rows and to the k rows:
+//   out[i] = rstd (x[i] w[i] cos - x[i + r/2] w[i + r/2] sin), and so on.
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -49,183 +53,264 @@ __device__ __forceinline__ int axis_of(const MropeArgs& a, int i) {
   return i < a.sec[0] ? 0 : i < a.sec[0] + a.sec[1] ? 1 : 2;
 }
 
-__device__ __forceinline__ double position_of(const MropeArgs& a, int axis, int64_t t) {
-  const int64_t at = axis * a.p_sa + t * a.p_st;
+__device__ __forceinline__ double position_at(const MropeArgs& a, int64_t at) {
   return a.pos64 ? static_cast<double>(static_cast<const int64_t*>(a.positions)[at])
                  : static_cast<double>(static_cast<const int32_t*>(a.positions)[at]);
 }
 
-// Rows read once. Not through the read-only path: q_out may be q.
-__device__ __forceinline__ uint4 ld_row(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p)
-               : "memory");
-  return v;
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
 
-// cos and sin of pos * freq: the product in turns, its whole part dropped, in 64 bits
-__device__ __forceinline__ void turn(double pos, float freq, float scaling, float* c, float* s) {
-  const double u = pos * (static_cast<double>(freq) * 0.15915494309189533577);
+// cos and sin of pos * turns a position: the product in turns, its whole part dropped, in
+// 64 bits
+__device__ __forceinline__ void turn(double pos, double turns, float scaling, float* c, float* s) {
+  const double u = pos * turns;
   sincospif(2.f * static_cast<float>(u - rint(u)), s, c);
   *c *= scaling;
   *s *= scaling;
 }
 
-// 8 values as e4m3 after a division by the scale (a true one: a product with the inverse
-// would fall on the other side of a border now and then).
-__device__ __forceinline__ uint2 pack8_e4m3(const float (&f)[8], float scale) {
+__device__ __forceinline__ uint2 pack8_e4m3(const float (&f)[8]) {
   uint32_t w[2] = {0, 0};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 x = make_float2(__fdiv_rn(f[2 * i], scale), __fdiv_rn(f[2 * i + 1], scale));
-    w[i / 2] |= static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(x, __NV_SATFINITE, __NV_E4M3))
+  for (int i = 0; i < 4; ++i)
+    w[i / 2] |= static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(
+                    make_float2(f[2 * i], f[2 * i + 1]), __NV_SATFINITE, __NV_E4M3))
                 << (i % 2 * 16);
-  }
   return make_uint2(w[0], w[1]);
 }
 
-constexpr int kThreads = 256;
-constexpr int kAhead = 2;  // row groups loaded before the first is used
+constexpr int kThreads = 256, kBlocksPerSm = 2;
+constexpr int kDepth = 4;  // row groups of a warp under way, 1 KB each
 
 template <int TPH, bool kE4m3>
-__global__ void __launch_bounds__(kThreads) mrope_kernel(MropeArgs a) {
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) mrope_kernel(MropeArgs a) {
+  __shared__ uint4 s_rows[kThreads / 32][kDepth][2][32];  // read by the lane that copied
   allow_dependent_launch();
   wait_prerequisite();
   constexpr int kRows = 32 / TPH;     // rows of a group
   constexpr int kShare = 8 / kRows;   // angles a lane makes (TPH >= 4, so at least one)
-  const int lane = threadIdx.x & 31, sub = lane % TPH, mine = lane / TPH;
-  const int64_t task = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
-  const int t = static_cast<int>(task / a.shares);
-  if (t >= a.tokens) return;
-  const int rows = a.hq + a.hk + (a.k_pages ? a.hk : 0);
-  const int row0 = static_cast<int>(task % a.shares) * a.groups * kRows;
-  const int row1 = min(rows, row0 + a.groups * kRows);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % TPH, mine = lane / TPH;
+  const unsigned worker = blockIdx.x * (kThreads / 32) + warp;
+  const int stride = gridDim.x * (kThreads / 32) / a.shares;  // tokens from one to the next
+  const int first = worker / a.shares;
+  if (first >= stride || first >= a.tokens) return;
+  const int g0 = worker % a.shares * a.groups;
+  const int k_from = (a.hq + kRows - 1) / kRows, v_from = k_from + (a.hk + kRows - 1) / kRows;
+  const int all = a.k_pages ? 2 * v_from - k_from : v_from;  // row groups, q before k before v
+  const int g1 = min(all, g0 + a.groups);
+  if (g0 >= g1) return;
 
   const int turned = a.half / 8;  // lanes of a row whose pairs are rotated
   const bool there = sub < a.d / 16, turns = sub < turned;
   const int lo = turns ? sub * 8 : 2 * a.half + (sub - turned) * 16;
   const int hi = turns ? a.half + sub * 8 : lo + 8;
-  const __nv_bfloat16* const q = a.q + t * a.q_st;
-  const __nv_bfloat16* const k = a.k + t * a.k_st;
-  const __nv_bfloat16* const v = a.v + t * a.v_st;
-  auto source = [&](int r) {
-    return r < a.hq ? q + r * a.q_sh
-           : r < a.hq + a.hk ? k + (r - a.hq) * a.k_sh : v + (r - a.hq - a.hk) * a.v_sh;
-  };
-  uint4 xl[kAhead], xh[kAhead];
-  auto fetch = [&](int first) {
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int r = first + u * kRows + mine;
-      xl[u] = xh[u] = make_uint4(0, 0, 0, 0);
-      if (there && r < row1) {
-        const __nv_bfloat16* p = source(r);
-        xl[u] = ld_row(p + lo);
-        xh[u] = ld_row(p + hi);
+
+  // ---- copies: the next group's token, place, and this lane's row of it
+  const uint32_t slot0 =
+      static_cast<uint32_t>(__cvta_generic_to_shared(&s_rows[warp][0][0][lane]));
+  int ct = first, cg = g0, cg_end = g0, crow = 0, cheads = 0;
+  const __nv_bfloat16* csrc = nullptr;
+  int64_t cstep = 0;
+  auto copy = [&](int stage) {
+    if (ct < a.tokens) {
+      if (cg == cg_end) {  // a kind of rows begins
+        const int from = cg < k_from ? 0 : cg < v_from ? k_from : v_from;
+        const int64_t sh = cg < k_from ? a.q_sh : cg < v_from ? a.k_sh : a.v_sh;
+        cg_end = min(g1, cg < k_from ? k_from : cg < v_from ? v_from : all);
+        cheads = !there ? 0 : cg < k_from ? a.hq : a.hk;
+        crow = (cg - from) * kRows + mine;
+        csrc = (cg < k_from ? a.q + ct * a.q_st : cg < v_from ? a.k + ct * a.k_st
+                                                              : a.v + ct * a.v_st) + crow * sh;
+        cstep = sh * kRows;
+      }
+      if (crow < cheads) {
+        copy16(slot0 + stage * 1024, csrc + lo);
+        copy16(slot0 + stage * 1024 + 512, csrc + hi);
+      }
+      csrc += cstep;
+      crow += kRows;
+      if (++cg == g1) {
+        cg = cg_end = g0;
+        ct += stride;
       }
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  fetch(row0);
+#pragma unroll
+  for (int i = 0; i < kDepth; ++i) copy(i);
+  int stage = 0;
+  auto take = [&](uint4& x, uint4& y) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+    x = s_rows[warp][stage][0][lane];
+    y = s_rows[warp][stage][1][lane];
+  };
+  auto give = [&]() {  // behind the last use of what take() gave
+    copy(stage);
+    stage = stage + 1 == kDepth ? 0 : stage + 1;
+  };
 
-  int64_t page_at = -1;  // where the token's K and V go; -1: nowhere
-  if (a.k_pages && row1 > a.hq) {
-    const int slot = a.slots[t];
-    if (slot >= 0 && slot < a.num_slots) {
-      const int page = slot / a.page_size;
-      page_at = page * a.pg_sp + (slot - page * a.page_size) * a.pg_ss;
-    } else if (slot != -1 && lane == 0) {
-      atomicOr(a.err, UMIC_DEVERR_BAD_PAGE);
+  // ---- this lane's share of a token's angles, and its slot, a token ahead
+  const bool angles = a.half && g0 < v_from, writes = a.k_pages && g1 > k_from;
+  double freq[kShare], pos[kShare];
+  int64_t pos_at[kShare];
+#pragma unroll
+  for (int x = 0; x < kShare; ++x) {
+    freq[x] = pos[x] = 0.;
+    pos_at[x] = 0;
+    const int i = min(sub * 8 + mine * kShare + x, a.half - 1);
+    if (angles) {
+      freq[x] = static_cast<double>(a.inv_freq[i]) * 0.15915494309189533577;
+      pos_at[x] = axis_of(a, i) * a.p_sa;
     }
   }
-  float c[8], s[8];
+  int slot = -1;
+  auto look = [&](int t) {
+    if (t >= a.tokens) return;
+    if (angles)
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    c[i] = s[i] = 0.f;
-  }
-  if (a.half && row0 < a.hq + a.hk) {
-    float mc[kShare], ms[kShare];
-#pragma unroll
-    for (int x = 0; x < kShare; ++x) {
-      const int i = min(sub * 8 + mine * kShare + x, a.half - 1);
-      turn(position_of(a, axis_of(a, i), t), a.inv_freq[i], a.scaling, &mc[x], &ms[x]);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int from = i / kShare * TPH + sub;
-      const float cv = __shfl_sync(0xffffffffu, mc[i % kShare], from);
-      const float sv = __shfl_sync(0xffffffffu, ms[i % kShare], from);
-      c[i] = cv;
-      s[i] = sv;
-    }
-  }
+      for (int x = 0; x < kShare; ++x) pos[x] = position_at(a, pos_at[x] + t * a.p_st);
+    if (writes) slot = a.slots[t];
+  };
+  look(first);
+  const float inv_d = 1.f / static_cast<float>(a.d);
 
 #pragma unroll 1
-  for (int first = row0; first < row1; first += kAhead * kRows) {
-    uint4 yl[kAhead], yh[kAhead];
+  for (int t = first; t < a.tokens; t += stride) {
+    float mc[kShare], ms[kShare];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      yl[u] = xl[u];
-      yh[u] = xh[u];
+    for (int x = 0; x < kShare; ++x) turn(pos[x], freq[x], a.scaling, &mc[x], &ms[x]);
+    int64_t page_at = -1;  // where the token's K and V go; -1: nowhere
+    if (writes && slot >= 0 && slot < a.num_slots) {
+      const int page = slot / a.page_size;
+      page_at = page * a.pg_sp + (slot - page * a.page_size) * a.pg_ss;
+    } else if (writes && slot != -1 && lane == 0) {
+      atomicOr(a.err, UMIC_DEVERR_BAD_PAGE);
     }
-    if (first + kAhead * kRows < row1) fetch(first + kAhead * kRows);
+    look(t + stride);
+
+#pragma unroll 1
+    for (int kind = g0 < k_from ? 0 : 1; kind < 2; ++kind) {  // q, k
+      const int from = kind ? k_from : 0, begin = max(g0, from);
+      const int end = min(g1, kind ? v_from : k_from);
+      if (begin >= end) continue;
+      const bool paged = kind && a.k_pages, e4m3 = kE4m3 && paged;
+      int row = (begin - from) * kRows + mine;
+      int64_t dst_step = paged ? a.pg_sh : kind ? a.ko_sh : a.qo_sh;
+      char* dst = static_cast<char*>(paged ? a.k_pages : kind ? a.k_out : a.q_out);
+      dst += ((paged ? page_at : t * (kind ? a.ko_st : a.qo_st)) + row * dst_step) *
+             (e4m3 ? 1 : 2);
+      dst_step *= e4m3 ? kRows : 2 * kRows;
+      const int heads = !there || (paged && page_at < 0) ? 0 : kind ? a.hk : a.hq;  // written
+      const void* wt = kind ? a.kw : a.qw;
+      const float eps = kind ? a.k_eps : a.q_eps;
+      // x' = x xc - y ys, y' = y yc + x xs; lanes past the rotated ones: x xc, y yc
+      float xc[8], ys[8], yc[8], xs[8];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int r = first + u * kRows + mine;
-      if (first + u * kRows >= row1) break;
-      const bool is_q = r < a.hq, is_v = r >= a.hq + a.hk;
-      const int h = is_q ? r : is_v ? r - a.hq - a.hk : r - a.hq;
-      float x[8], y[8];
-      unpack8(yl[u], x);
-      unpack8(yh[u], y);
-      if (a.qw || a.kw) {  // all lanes take part in the shuffles
-        float ss = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) ss += x[i] * x[i] + y[i] * y[i];
-#pragma unroll
-        for (int o = TPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const void* w = is_q ? a.qw : is_v ? nullptr : a.kw;
-        if (w && there) {
-          const float rstd = rsqrtf(ss / static_cast<float>(a.d) + (is_q ? a.q_eps : a.k_eps));
-          float wv[8];
-          load_w8(w, a.w_dtype, lo, wv);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = x[i] * rstd * wv[i];
-          load_w8(w, a.w_dtype, hi, wv);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = y[i] * rstd * wv[i];
-        }
+      for (int i = 0; i < 8; ++i) xc[i] = yc[i] = 1.f;
+      if (wt && there) {
+        load_w8(wt, a.w_dtype, lo, xc);
+        load_w8(wt, a.w_dtype, hi, yc);
       }
-      const bool plain = is_v || !turns;  // not "times 1 plus times 0": infinity passes
-      float ox[8], oy[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        ox[i] = plain ? x[i] : x[i] * c[i] - y[i] * s[i];
-        oy[i] = plain ? y[i] : y[i] * c[i] + x[i] * s[i];
-      }
-      if (!there || r >= row1) continue;
-      if (is_q || !a.k_pages) {
-        __nv_bfloat16* out =
-            is_q ? a.q_out + t * a.qo_st + h * a.qo_sh : a.k_out + t * a.ko_st + h * a.ko_sh;
-        st_vec(out + lo, pack8(ox));
-        st_vec(out + hi, pack8(oy));
-      } else if (page_at >= 0) {
-        const int64_t at = page_at + h * a.pg_sh;
-        if constexpr (kE4m3) {
-          const float* scales = is_v ? a.v_scale : a.k_scale;
-          const float scale = scales ? __ldg(scales + h) : 1.f;
-          uint8_t* out = static_cast<uint8_t*>(is_v ? a.v_pages : a.k_pages) + at;
-          *reinterpret_cast<uint2*>(out + lo) = pack8_e4m3(ox, scale);
-          *reinterpret_cast<uint2*>(out + hi) = pack8_e4m3(oy, scale);
-        } else {
-          __nv_bfloat16* out = static_cast<__nv_bfloat16*>(is_v ? a.v_pages : a.k_pages) + at;
-          st_vec(out + lo, pack8(ox));
-          st_vec(out + hi, pack8(oy));
+        const int src = i / kShare * TPH + sub;
+        const float c = __shfl_sync(0xffffffffu, mc[i % kShare], src);
+        const float s = __shfl_sync(0xffffffffu, ms[i % kShare], src);
+        ys[i] = yc[i] * s;
+        xs[i] = xc[i] * s;
+        if (turns) {
+          xc[i] *= c;
+          yc[i] *= c;
         }
       }
+#pragma unroll 1
+      for (int left = end - begin; left > 0; --left) {
+        uint4 xv, yv;
+        take(xv, yv);
+        float x[8], y[8];
+        unpack8(xv, x);
+        unpack8(yv, y);
+        float f = 1.f;
+        if (wt) {
+          float ss = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) ss += x[i] * x[i] + y[i] * y[i];
+          if (!there || row >= (kind ? a.hk : a.hq)) ss = 0.f;  // pieces not copied
+#pragma unroll
+          for (int o = TPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          f = rsqrtf(ss * inv_d + eps);
+        }
+        if (e4m3 && a.k_scale && row < a.hk) f /= __ldg(a.k_scale + row);
+        if (turns) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float u = x[i] * xc[i] - y[i] * ys[i];
+            y[i] = y[i] * yc[i] + x[i] * xs[i];
+            x[i] = u;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            x[i] *= xc[i];
+            y[i] *= yc[i];
+          }
+        }
+        if (wt || e4m3) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            x[i] *= f;
+            y[i] *= f;
+          }
+        }
+        if (row < heads) {
+          if (e4m3) {
+            *reinterpret_cast<uint2*>(dst + lo) = pack8_e4m3(x);
+            *reinterpret_cast<uint2*>(dst + hi) = pack8_e4m3(y);
+          } else {
+            st_vec(dst + 2 * lo, pack8(x));
+            st_vec(dst + 2 * hi, pack8(y));
+          }
+        }
+        dst += dst_step;
+        row += kRows;
+        give();
+      }
+    }
+    // v: a copy, or a rounding to e4m3
+    const int begin = max(g0, v_from);
+    int row = (begin - v_from) * kRows + mine;
+    char* dst = static_cast<char*>(a.v_pages) + (page_at + row * a.pg_sh) * (kE4m3 ? 1 : 2);
+    const int heads = there && page_at >= 0 ? a.hk : 0;
+#pragma unroll 1
+    for (int left = g1 - begin; left > 0; --left) {
+      uint4 xv, yv;
+      take(xv, yv);
+      if (row < heads) {
+        if constexpr (kE4m3) {
+          float x[8], y[8];
+          unpack8(xv, x);
+          unpack8(yv, y);
+          const float f = a.v_scale ? 1.f / __ldg(a.v_scale + row) : 1.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            x[i] *= f;
+            y[i] *= f;
+          }
+          *reinterpret_cast<uint2*>(dst + lo) = pack8_e4m3(x);
+          *reinterpret_cast<uint2*>(dst + hi) = pack8_e4m3(y);
+        } else {
+          st_vec(dst + 2 * lo, xv);
+          st_vec(dst + 2 * hi, yv);
+        }
+      }
+      dst += a.pg_sh * (kE4m3 ? kRows : 2 * kRows);
+      row += kRows;
+      give();
     }
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 template <int TPH>
@@ -333,18 +418,30 @@ extern "C" int umic_qk_norm_mrope_kv(
   a.q_eps = q_eps;
   a.k_eps = k_eps;
   a.scaling = scaling;
-  const int64_t rows = static_cast<int64_t>(hq) + hk + (k_pages ? hk : 0);
-  const int tph = head_dim <= 64 ? 4 : head_dim <= 128 ? 8 : 16;
-  const int64_t groups = (rows + 32 / tph - 1) / (32 / tph);
-  // A warp each for a row group while that leaves the GPU's warps (64 an SM) unfilled; with
-  // more tokens longer shares, which make a token's angles fewer times.
-  const int64_t per = tokens * groups / (static_cast<int64_t>(sm_count()) * 64);
-  a.groups = static_cast<int32_t>(std::max<int64_t>(1, std::min(per, groups)));
-  a.shares = static_cast<int32_t>((groups + a.groups - 1) / a.groups);
-  const int64_t blocks = (tokens * a.shares + kThreads / 32 - 1) / (kThreads / 32);
-  if (blocks > 0x7fffffffLL)
-    return fail(UMIC_ERR_UNSUPPORTED, "%s: %lld tokens x %lld heads", me, (long long)tokens,
-                (long long)rows);
+  const int tph = head_dim <= 64 ? 4 : head_dim <= 128 ? 8 : 16, at_once = 32 / tph;
+  const int64_t groups = (static_cast<int64_t>(hq) + at_once - 1) / at_once +
+                         (static_cast<int64_t>(hk) + at_once - 1) / at_once * (k_pages ? 2 : 1);
+  if (groups > (1 << 20))
+    return fail(UMIC_ERR_UNSUPPORTED, "%s: too many heads (%d + %d)", me, hq, hk);
+  // A token's row groups go to one warp or are shared by several: the fewest rounds of
+  // groups, with two more for a token's angles and start, that the GPU's resident warps
+  // need for all tokens.
+  const int64_t warps = static_cast<int64_t>(sm_count()) * kBlocksPerSm * (kThreads / 32);
+  int64_t best = INT64_MAX;
+  for (int64_t per = groups; per >= 1; per = per > 16 ? per / 2 : per - 1) {
+    const int64_t shares = (groups + per - 1) / per;
+    const int64_t rounds = (tokens * shares + warps - 1) / warps * (per + 2);
+    if (rounds < best) {
+      best = rounds;
+      a.groups = static_cast<int32_t>(per);
+      a.shares = static_cast<int32_t>(shares);
+    }
+  }
+  const int64_t wanted = (tokens * a.shares + kThreads / 32 - 1) / (kThreads / 32);
+  // at least a token's shares
+  const int64_t blocks =
+      std::max<int64_t>(std::min<int64_t>(wanted, sm_count() * kBlocksPerSm),
+                        (a.shares + kThreads / 32 - 1) / (kThreads / 32));
   cudaStream_t st = as_stream(stream);
   if (tph == 4) launch<4>(a, blocks, st);
   else if (tph == 8) launch<8>(a, blocks, st);
