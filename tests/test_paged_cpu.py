@@ -186,3 +186,12 @@ def test_wrappers_refuse_cpu_tensors():
     with pytest.raises(RuntimeError, match="no CPU path"):
         paged_attention(x, pages, pages, _z(3, 2, dtype=torch.int32), _z(3, dtype=torch.int32),
                         0.1)
+
+
+def test_paged_cache_refuses_other_slabs():
+    from umic_b200.paged import PagedKVCache
+
+    with pytest.raises(ValueError, match="slab"):
+        PagedKVCache(_z(2, 3, 4, 2, 16, 64), 2, 3)
+    with pytest.raises(ValueError, match="slab"):
+        PagedKVCache(_z(2, 4, 2, 16, 64), 2, 3)
