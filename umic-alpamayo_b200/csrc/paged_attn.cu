@@ -815,12 +815,15 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
 
   // ---- join the tails of this CTA: a run of warps from one that is not continued from its
   // left neighbour to the last one that continues it
-  for (int w0 = 0; w0 < kWarps; ++w0) {
+  const int flags = lane < kWarps ? s_tail[lane].x : 0;
+  const unsigned has = __ballot_sync(0xffffffffu, flags & 1);
+  const unsigned first_tile = __ballot_sync(0xffffffffu, flags & 2);
+  const unsigned last_tile = __ballot_sync(0xffffffffu, flags & 4);
+  for (unsigned heads = has & (first_tile | 1u); heads; heads &= heads - 1) {
+    const int w0 = __ffs(heads) - 1;
+    const int w1 = w0 + __ffs(~((has & ~first_tile) >> (w0 + 1))) - 1;
     const int4 head = s_tail[w0];
-    if (!(head.x & 1) || (w0 > 0 && !(head.x & 2))) continue;
-    int w1 = w0;
-    while (w1 + 1 < kWarps && (s_tail[w1 + 1].x & 3) == 1) ++w1;
-    const bool whole = (head.x & 2) && (s_tail[w1].x & 4);
+    const bool whole = (first_tile >> w0 & 1) && (last_tile >> w1 & 1);
     float* const slot = a.ws.slot(first_worker + w0, 0, S::kSlot);
     for (int at = warp; at < NT * kBlocks; at += kWarps) {
       const int nt = at / kBlocks, k = at % kBlocks;

@@ -14,6 +14,7 @@ step. `PagedKVCache` (umic_b200.paged) keeps the pool and runs them together.
 
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple
 
 import torch
@@ -256,6 +257,12 @@ def paged_kv_append(k_pages: torch.Tensor, v_pages: torch.Tensor, k_new: torch.T
     stats["umic_paged_kv_append"] += 1
 
 
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(dev: torch.device, *sizes: int) -> int:
+    _lib._ensure_device(dev)
+    return _lib.lib().umic_paged_attention_workspace_bytes(*sizes)
+
+
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                     block_table: torch.Tensor, kv_lens: torch.Tensor, scale: float, *,
                     k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
@@ -284,8 +291,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     lse = torch.empty((b, hq), dtype=torch.float32, device=dev) if return_lse else None
     # its own workspace for every call: calls on several streams, and graphs captured
     # apart, never share one
-    _lib._ensure_device(dev)
-    need = _lib.lib().umic_paged_attention_workspace_bytes(b, hq, hk, d, width, page, dt)
+    need = _workspace_bytes(dev, b, hq, hk, d, width, page, dt)
     ws = q.new_empty((need + 1) // 2)
     _lib.call("umic_paged_attention", dev, qa[0], qa[1], qa[2], k_pages.data_ptr(),
               v_pages.data_ptr(), sp, sh, ss, p, page, dt, _lib.ptr(k_scale),
