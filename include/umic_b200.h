@@ -206,7 +206,8 @@ UMIC_API int umic_qk_norm_rope_kv(
  * pg_sh, pg_ss) element strides, K and V with the same strides, bf16 or e4m3 (with one
  * fp32 scale per KV head: value = stored * scale; NULL = 1). A request's tokens
  * [i * page_size, (i + 1) * page_size) live in page block_table[request, i]; the slot
- * of a token is page * page_size + its place in the page. No reference counterpart:
+ * of a token is page * page_size + its place in the page. Two of the calls take their
+ * arguments, which are many, as a struct. No reference counterpart:
  * the reference keeps one dense buffer per layer whose rows share a length
  * (src/umic/cache.py:25-160). */
 
@@ -258,17 +259,22 @@ UMIC_API int umic_paged_plan(const int32_t* kv_lens, const int32_t* new_tokens,
  * cos/sin tables of transformers' rotary module, apply_rotary_pos_emb (rope.py:86-107)
  * or apply_rotary_vision_triton (rope.py:78-84), and the cache write
  * (cache.py:59-60). */
-UMIC_API int umic_qk_norm_mrope_kv(
-    const void* q, int64_t q_st, int64_t q_sh, int32_t hq, const void* k, int64_t k_st,
-    int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, int32_t hk, void* q_out,
-    int64_t qo_st, int64_t qo_sh, void* k_out, int64_t ko_st, int64_t ko_sh,
-    const void* q_weight, const void* k_weight, int w_dtype, float q_eps, float k_eps,
-    const void* positions, int pos_bytes, int64_t p_sa, int64_t p_st, const float* inv_freq,
-    int32_t rotary_dim, int32_t axes, int32_t s0, int32_t s1, int32_t s2, int interleaved,
-    float scaling, void* k_pages, void* v_pages, int64_t pg_sp, int64_t pg_sh, int64_t pg_ss,
-    int64_t num_pages, int64_t page_size, int cache_dtype, const float* k_scale,
-    const float* v_scale, const int32_t* slots, int64_t tokens, int32_t head_dim,
-    void* stream);
+typedef struct umic_mrope_args {
+  const void *q, *k, *v;
+  void *q_out, *k_out;
+  const void *q_weight, *k_weight; /* [head_dim], w_dtype */
+  const void* positions;
+  const float* inv_freq;           /* [rotary_dim / 2] */
+  void *k_pages, *v_pages;
+  const float *k_scale, *v_scale;  /* [hk] */
+  const int32_t* slots;            /* [tokens] */
+  int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, qo_st, qo_sh, ko_st, ko_sh;
+  int64_t p_sa, p_st, pg_sp, pg_sh, pg_ss, num_pages, page_size, tokens;
+  int32_t hq, hk, head_dim, w_dtype, pos_bytes, rotary_dim, axes, s0, s1, s2, interleaved;
+  int32_t cache_dtype;
+  float q_eps, k_eps, scaling;
+} umic_mrope_args;
+UMIC_API int umic_qk_norm_mrope_kv(const umic_mrope_args* args, void* stream);
 
 /* Attention of one new token per request over its pages, grouped-query heads:
  * out[b, h] = softmax(scale * q[b, h] . k_j over j < kv_lens[b]) . v_j. q and out
@@ -283,13 +289,19 @@ UMIC_API int umic_qk_norm_mrope_kv(
  * irrelevant before and after; calls that may overlap need one each.
  * Replaces the SDPA call of the decode step (graph.py:76-99), for rows of different
  * lengths. */
-UMIC_API int umic_paged_attention(
-    const void* q, int64_t q_sb, int64_t q_sh, const void* k_pages, const void* v_pages,
-    int64_t pg_sp, int64_t pg_sh, int64_t pg_ss, int64_t num_pages, int64_t page_size,
-    int cache_dtype, const float* k_scale, const float* v_scale, const int32_t* block_table,
-    int64_t table_stride, int64_t max_pages, const int32_t* kv_lens, void* out, int64_t o_sb,
-    int64_t o_sh, float* lse, int64_t batch, int32_t hq, int32_t hkv, int32_t head_dim,
-    float scale, void* workspace, size_t workspace_bytes, void* stream);
+typedef struct umic_paged_attention_args {
+  const void *q, *k_pages, *v_pages;
+  const float *k_scale, *v_scale; /* [hkv] */
+  const int32_t *block_table, *kv_lens;
+  void* out;
+  float* lse;
+  void* workspace;
+  int64_t q_sb, q_sh, pg_sp, pg_sh, pg_ss, num_pages, page_size, table_stride, max_pages;
+  int64_t o_sb, o_sh, batch, workspace_bytes;
+  int32_t hq, hkv, head_dim, cache_dtype;
+  float scale;
+} umic_paged_attention_args;
+UMIC_API int umic_paged_attention(const umic_paged_attention_args* args, void* stream);
 
 /* Bytes of workspace umic_paged_attention needs for these sizes on the current device,
  * whatever the lengths. */

@@ -12,7 +12,6 @@ from umic_b200 import _lib
 from umic_b200.kernels import (paged_attention, paged_kv_append, paged_plan, qk_norm_mrope_kv)
 
 F = ctypes.c_void_p(4096)  # never dereferenced: the check under test fails first
-f32 = ctypes.c_float
 
 
 # ------------------------------------------------------------------- oracle
@@ -109,13 +108,18 @@ def test_plan_refusals(kw, code, text):
     assert text in _lib.last_message()
 
 
+def _at(p):
+    return 0 if p is None else p.value
+
+
 def _mrope(q=F, q_st=512, hq=4, k=F, k_st=256, v=F, hk=2, k_out=None, w=0, positions=F, pos=8,
            rot=128, axes=3, sec=(24, 20, 20), kp=F, pg=(8192, 2048, 128), num=8, page=16, dt=0,
            slots=F, tokens=4, d=128):
-    return _lib.lib().umic_qk_norm_mrope_kv(
-        q, q_st, d, hq, k, k_st, d, v, k_st, d, hk, F, 512, d, k_out, 256, d, None, None, w,
-        f32(1e-6), f32(1e-6), positions, pos, 4, 1, F, rot, axes, *sec, 1, f32(1.0), kp, kp, *pg,
-        num, page, dt, None, None, slots, tokens, d, None)
+    args = _lib.pack_mrope_args(
+        _at(q), _at(k), _at(v), _at(F), _at(k_out), 0, 0, _at(positions), _at(F), _at(kp),
+        _at(kp), 0, 0, _at(slots), q_st, d, k_st, d, k_st, d, 512, d, 256, d, 4, 1, *pg, num,
+        page, tokens, hq, hk, d, w, pos, rot, axes, *sec, 1, dt, 1e-6, 1e-6, 1.0)
+    return _lib.lib().umic_qk_norm_mrope_kv(args, None)
 
 
 @pytest.mark.parametrize("kw,code,text", [
@@ -139,13 +143,34 @@ def test_input_refusals(kw, code, text):
 
 def test_input_of_no_tokens_is_a_noop():
     assert _mrope(tokens=0, q=None, k=None) == 0
+    assert _lib.lib().umic_qk_norm_mrope_kv(None, None) == 1
 
 
 def _attend(q=F, q_sb=512, kp=F, pg=(8192, 2048, 128), num=8, page=16, dt=0, table=F, width=4,
             lens=F, out=F, batch=2, hq=4, hk=2, d=128, ws=F, ws_bytes=1 << 30):
-    return _lib.lib().umic_paged_attention(
-        q, q_sb, 128, kp, kp, *pg, num, page, dt, None, None, table, width, width, lens, out, 512,
-        128, None, batch, hq, hk, d, f32(0.1), ws, ws_bytes, None)
+    args = _lib.pack_paged_attention_args(
+        _at(q), _at(kp), _at(kp), 0, 0, _at(table), _at(lens), _at(out), 0, _at(ws), q_sb, 128,
+        *pg, num, page, width, width, 512, 128, batch, ws_bytes, hq, hk, d, dt, 0.1)
+    return _lib.lib().umic_paged_attention(args, None)
+
+
+def test_structs_match_the_header():
+    """The packed formats against the header's fields, in order and by type."""
+    import re
+    from pathlib import Path
+
+    header = (Path(__file__).resolve().parent.parent / "include" / "umic_b200.h").read_text()
+    for name, fmt in (("umic_mrope_args", "14Q18q12i3f"), ("umic_paged_attention_args",
+                                                          "10Q13q4if")):
+        body = re.search(r"typedef struct " + name + r" \{(.*?)\} " + name + ";", header,
+                         re.S).group(1)
+        kinds = ""
+        for line in re.sub(r"/\*.*?\*/", "", body, flags=re.S).split(";"):
+            n = len(line.split(",")) if line.strip() else 0
+            kind = "Q" if "*" in line else "q" if "int64_t" in line else \
+                "i" if "int32_t" in line else "f"
+            kinds += kind * n
+        assert kinds == "".join(c * int(n or 1) for n, c in re.findall(r"(\d*)([Qqif])", fmt))
 
 
 @pytest.mark.parametrize("kw,code,text", [
@@ -166,6 +191,7 @@ def test_attend_refusals(kw, code, text):
 
 def test_attend_of_no_requests_is_a_noop():
     assert _attend(batch=0, q=None) == 0
+    assert _lib.lib().umic_paged_attention(None, None) == 1
 
 
 # -------------------------------------------------------- wrapper refusals

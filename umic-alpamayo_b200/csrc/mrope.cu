@@ -325,19 +325,15 @@ void launch(const MropeArgs& a, int64_t blocks, cudaStream_t st) {
 
 using namespace umic;
 
-extern "C" int umic_qk_norm_mrope_kv(
-    const void* q, int64_t q_st, int64_t q_sh, int32_t hq, const void* k, int64_t k_st,
-    int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, int32_t hk, void* q_out,
-    int64_t qo_st, int64_t qo_sh, void* k_out, int64_t ko_st, int64_t ko_sh,
-    const void* q_weight, const void* k_weight, int w_dtype, float q_eps, float k_eps,
-    const void* positions, int pos_bytes, int64_t p_sa, int64_t p_st, const float* inv_freq,
-    int32_t rotary_dim, int32_t axes, int32_t s0, int32_t s1, int32_t s2, int interleaved,
-    float scaling, void* k_pages, void* v_pages, int64_t pg_sp, int64_t pg_sh, int64_t pg_ss,
-    int64_t num_pages, int64_t page_size, int cache_dtype, const float* k_scale,
-    const float* v_scale, const int32_t* slots, int64_t tokens, int32_t head_dim,
-    void* stream) {
+extern "C" int umic_qk_norm_mrope_kv(const umic_mrope_args* args, void* stream) {
   const char* const me = "umic_qk_norm_mrope_kv";
   clear_error();
+  if (!args) return fail(UMIC_ERR_INVALID_ARG, "%s: null pointer", me);
+  const auto& [q, k, v, q_out, k_out, q_weight, k_weight, positions, inv_freq, k_pages,
+               v_pages, k_scale, v_scale, slots, q_st, q_sh, k_st, k_sh, v_st, v_sh, qo_st,
+               qo_sh, ko_st, ko_sh, p_sa, p_st, pg_sp, pg_sh, pg_ss, num_pages, page_size,
+               tokens, hq, hk, head_dim, w_dtype, pos_bytes, rotary_dim, axes, s0, s1, s2,
+               interleaved, cache_dtype, q_eps, k_eps, scaling] = *args;
   if (hq < 0 || hk <= 0 || tokens < 0 || head_dim <= 0)
     return fail(UMIC_ERR_INVALID_ARG, "%s: hq=%d hk=%d tokens=%lld head_dim=%d", me, hq, hk,
                 (long long)tokens, head_dim);

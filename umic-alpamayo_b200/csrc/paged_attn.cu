@@ -1073,15 +1073,14 @@ extern "C" size_t umic_paged_attention_workspace_bytes(int64_t batch, int32_t hq
                       per * (head_dim + 2));
 }
 
-extern "C" int umic_paged_attention(
-    const void* q, int64_t q_sb, int64_t q_sh, const void* k_pages, const void* v_pages,
-    int64_t pg_sp, int64_t pg_sh, int64_t pg_ss, int64_t num_pages, int64_t page_size,
-    int cache_dtype, const float* k_scale, const float* v_scale, const int32_t* block_table,
-    int64_t table_stride, int64_t max_pages, const int32_t* kv_lens, void* out, int64_t o_sb,
-    int64_t o_sh, float* lse, int64_t batch, int32_t hq, int32_t hkv, int32_t head_dim,
-    float scale, void* workspace, size_t workspace_bytes, void* stream) {
+extern "C" int umic_paged_attention(const umic_paged_attention_args* args, void* stream) {
   const char* const me = "umic_paged_attention";
   clear_error();
+  if (!args) return fail(UMIC_ERR_INVALID_ARG, "%s: null pointer", me);
+  const auto& [q, k_pages, v_pages, k_scale, v_scale, block_table, kv_lens, out, lse,
+               workspace, q_sb, q_sh, pg_sp, pg_sh, pg_ss, num_pages, page_size,
+               table_stride, max_pages, o_sb, o_sh, batch, workspace_bytes, hq, hkv,
+               head_dim, cache_dtype, scale] = *args;
   if (batch < 0 || hq <= 0 || hkv <= 0 || num_pages <= 0 || page_size <= 0 || max_pages < 0)
     return fail(UMIC_ERR_INVALID_ARG,
                 "%s: batch=%lld hq=%d hkv=%d num_pages=%lld page_size=%lld max_pages=%lld", me,
@@ -1116,9 +1115,9 @@ extern "C" int umic_paged_attention(
     return fail(UMIC_ERR_ALIGNMENT, "%s: 16-byte alignment of bases / strides", me);
   const size_t need = umic_paged_attention_workspace_bytes(batch, hq, hkv, head_dim, max_pages,
                                                            page_size, cache_dtype);
-  if (!workspace || !aligned16(workspace) || workspace_bytes < need)
-    return fail(UMIC_ERR_INVALID_ARG, "%s: workspace of %zu bytes (%zu needed, 16-byte aligned)",
-                me, workspace_bytes, need);
+  if (!workspace || !aligned16(workspace) || workspace_bytes < static_cast<int64_t>(need))
+    return fail(UMIC_ERR_INVALID_ARG, "%s: workspace of %lld bytes (%zu needed, 16-byte aligned)",
+                me, (long long)workspace_bytes, need);
   uint32_t* err = device_error_word();
   if (!err) return fail(UMIC_ERR_DEVICE, "%s: no device error word", me);
   const bool e4m3 = cache_dtype == UMIC_DTYPE_E4M3;

@@ -10,6 +10,7 @@ if the library is missing or fails to load, the first kernel call raises.
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from pathlib import Path
 
@@ -71,16 +72,8 @@ _SIGNATURES: dict[str, list] = {
                             _c_i64, _c_i64, _c_i64, _c_p],
     "umic_paged_plan": [_c_p, _c_p, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_i64,
                         _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_p],
-    "umic_qk_norm_mrope_kv": [_c_p, _c_i64, _c_i64, _c_i32, _c_p, _c_i64, _c_i64, _c_p, _c_i64,
-                              _c_i64, _c_i32, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p,
-                              _c_p, _c_int, _c_f32, _c_f32, _c_p, _c_int, _c_i64, _c_i64, _c_p,
-                              _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_int, _c_f32, _c_p, _c_p,
-                              _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_int, _c_p, _c_p, _c_p,
-                              _c_i64, _c_i32, _c_p],
-    "umic_paged_attention": [_c_p, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64,
-                             _c_i64, _c_int, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p,
-                             _c_i64, _c_i64, _c_p, _c_i64, _c_i32, _c_i32, _c_i32, _c_f32, _c_p,
-                             _c_size, _c_p],
+    "umic_qk_norm_mrope_kv": [_c_p, _c_p],
+    "umic_paged_attention": [_c_p, _c_p],
     "umic_paged_attention_workspace_bytes": [_c_i64, _c_i32, _c_i32, _c_i32, _c_i64, _c_i64,
                                              _c_int],
     "umic_gemm": [_c_p, _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_i64, _c_p, _c_i64, _c_i64, _c_i64,
@@ -94,6 +87,11 @@ _SIGNATURES: dict[str, list] = {
 _RESTYPES = {"umic_last_error_message": ctypes.c_char_p, "umic_gemv_workspace_bytes": _c_size,
              "umic_gemm_workspace_bytes": _c_size,
              "umic_paged_attention_workspace_bytes": _c_size}
+
+# umic_mrope_args and umic_paged_attention_args as bytes, fields in the header's order
+# (packing costs a fifth of what ctypes takes to convert as many arguments)
+pack_mrope_args = struct.Struct("@14Q18q12i3f").pack
+pack_paged_attention_args = struct.Struct("@10Q13q4if").pack
 
 ERR_NAMES = {1: "INVALID_ARG", 2: "UNSUPPORTED", 3: "ALIGNMENT", 4: "LAUNCH", 5: "OVERFLOW",
              6: "DEVICE"}

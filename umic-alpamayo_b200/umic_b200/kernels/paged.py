@@ -15,6 +15,7 @@ step. `PagedKVCache` (umic_b200.paged) keeps the pool and runs them together.
 from __future__ import annotations
 
 import functools
+import struct
 from typing import NamedTuple
 
 import torch
@@ -153,66 +154,89 @@ def _input(name, q, k, v, positions, inv_freq, sections, interleaved, scaling, q
            k_weight, q_eps, k_eps, k_pages, v_pages, slots, k_scale, v_scale, q_out, k_out):
     dev = _one_device(name, k, q, v, positions, inv_freq, q_weight, k_weight, k_pages, v_pages,
                       slots, k_scale, v_scale, q_out, k_out)
-    if k.ndim != 3:
-        raise ValueError(f"{name}: k must be [tokens, heads, head_dim], got {tuple(k.shape)}")
-    t, hk, d = k.shape
-    ka = _rows(name, "k", k, t, hk, d)
-    va = (None, 0, 0) if v is None else _rows(name, "v", v, t, hk, d)[:3]
+    shape, strides = k.shape, k.stride()
+    if len(shape) != 3:
+        raise ValueError(f"{name}: k must be [tokens, heads, head_dim], got {tuple(shape)}")
+    t, hk, d = shape
+    if k.dtype is not torch.bfloat16 or strides[2] != 1:
+        _rows(name, "k", k, t, hk, d)
+    k_st, k_sh, _ = strides
+    if v is None:
+        v_ptr = v_st = v_sh = 0
+    else:
+        v_ptr, v_st, v_sh, _ = _rows(name, "v", v, t, hk, d)
+    kp = vp = pg_sp = pg_sh = pg_ss = num_pages = page = ks = vs = slots_ptr = 0
+    ko = ko_st = ko_sh = 0
+    dt = _lib.DTYPE_BF16
     if k_pages is None:
         if v_pages is not None or slots is not None or k_scale is not None or \
                 v_scale is not None:
             raise ValueError(f"{name}: v_pages, slots and scales go with k_pages")
         if k_out is None:
-            k_out = k.new_empty((t, hk, d))
-        ko = _rows(name, "k_out", k_out, t, hk, d)[:3]
-        pool = (None, None, 0, 0, 0, 0, 0, _lib.DTYPE_BF16, None, None, None)
+            k_out = k.new_empty(shape)
+        ko, ko_st, ko_sh, _ = _rows(name, "k_out", k_out, t, hk, d)
     else:
         if v is None or v_pages is None or slots is None:
             raise ValueError(f"{name}: a cache write needs v, v_pages and slots")
         if k_out is not None:
             raise ValueError(f"{name}: k_out goes without k_pages")
-        dt, shape, strides = _check_pages(name, k_pages, v_pages, k_scale, v_scale)
-        if shape[1] != hk or shape[3] != d:
-            raise ValueError(f"{name}: pages {tuple(shape)} do not match k {tuple(k.shape)}")
+        dt, (num_pages, heads, page, dim), (pg_sp, pg_sh, pg_ss, _) = _check_pages(
+            name, k_pages, v_pages, k_scale, v_scale)
+        if heads != hk or dim != d:
+            raise ValueError(f"{name}: pages {tuple(k_pages.shape)} do not match k "
+                             f"{tuple(shape)}")
         _require(name, "slots", slots, torch.int32, t)
-        pool = (k_pages.data_ptr(), v_pages.data_ptr(), strides[0], strides[1], strides[2],
-                shape[0], shape[2], dt, _lib.ptr(k_scale), _lib.ptr(v_scale), slots.data_ptr())
-        ko = (None, 0, 0)
+        kp, vp, slots_ptr = k_pages.data_ptr(), v_pages.data_ptr(), slots.data_ptr()
+        if k_scale is not None:
+            ks = k_scale.data_ptr()
+        if v_scale is not None:
+            vs = v_scale.data_ptr()
     if q is None:
-        qa, qo = (None, 0, 0, 0), (None, 0, 0)
+        q_ptr = q_st = q_sh = hq = qo = qo_st = qo_sh = 0
     else:
-        qa = _rows(name, "q", q, t, None, d)
+        q_ptr, q_st, q_sh, hq = _rows(name, "q", q, t, None, d)
         if q_out is None:
-            q_out = q.new_empty((t, qa[3], d))
-        qo = _rows(name, "q_out", q_out, t, qa[3], d)[:3]
-    wdt = _lib.DTYPE_BF16
-    if q_weight is not None or k_weight is not None:
-        w = q_weight if q_weight is not None else k_weight
-        wdt = _w_dtype(w)
-        _require(name, "q_weight", w, w.dtype, d)
-        if k_weight is not None:
-            _require(name, "k_weight", k_weight, w.dtype, d)
-    if positions is None:
-        rot = (None, 4, 0, 0, None, 0, 1, 0, 0, 0, 0)
-    else:
-        axes, (p_sa, p_st) = 1, (0, 1)
-        if positions.ndim == 2:
-            axes, (p_sa, p_st) = positions.shape[0], positions.stride()
-        elif positions.ndim == 1:
-            p_st = positions.stride(0)
-        if positions.dtype not in (torch.int32, torch.int64) or positions.ndim not in (1, 2) or \
-                positions.shape[-1] != t or not 1 <= axes <= 3 or len(sections) != axes:
+            q_out = q.new_empty((t, hq, d))
+            qo, qo_st, qo_sh = q_out.data_ptr(), hq * d, d
+        else:
+            qo, qo_st, qo_sh, _ = _rows(name, "q_out", q_out, t, hq, d)
+    qw = kw = wdt = 0
+    if q_weight is not None:
+        wdt = _w_dtype(q_weight)
+        _require(name, "q_weight", q_weight, q_weight.dtype, d)
+        qw = q_weight.data_ptr()
+    if k_weight is not None:
+        wdt = _w_dtype(k_weight)
+        _require(name, "k_weight", k_weight, k_weight.dtype if qw == 0 else q_weight.dtype, d)
+        kw = k_weight.data_ptr()
+    pos = inv = p_sa = p_st = s0 = s1 = s2 = half = 0
+    pos_bytes = axes = 1
+    if positions is not None:
+        p_shape, dtype, n = positions.shape, positions.dtype, len(sections)
+        pos_bytes = 8 if dtype is torch.int64 else 4
+        if p_shape == (n, t):
+            axes, (p_sa, p_st) = n, positions.stride()
+        elif n == 1 and p_shape == (t,):
+            p_st, = positions.stride()
+        else:
+            axes = 0
+        if not 1 <= axes <= 3 or (dtype is not torch.int64 and dtype is not torch.int32):
             raise ValueError(f"{name}: positions must be int32 or int64 [axes, {t}] with one of "
-                             f"{len(sections)} sections per axis (1 to 3), got "
-                             f"{positions.dtype} {tuple(positions.shape)}")
+                             f"{n} sections per axis (1 to 3), got {dtype} {tuple(p_shape)}")
         half = inv_freq.numel()
         _require(name, "inv_freq", inv_freq, torch.float32, half)
         s0, s1, s2 = (*sections, 0, 0)[:3]
-        rot = (positions.data_ptr(), 4 if positions.dtype is torch.int32 else 8, p_sa, p_st,
-               inv_freq.data_ptr(), 2 * half, axes, s0, s1, s2, int(interleaved))
-    _lib.call("umic_qk_norm_mrope_kv", dev, *qa, *ka[:3], *va, hk, *qo, *ko, _lib.ptr(q_weight),
-              _lib.ptr(k_weight), wdt, q_eps, k_eps, *rot, scaling, *pool, t, d)
-    return q_out, (k_out if k_pages is None else None)
+        pos, inv = positions.data_ptr(), inv_freq.data_ptr()
+    try:
+        args = _lib.pack_mrope_args(
+            q_ptr, k.data_ptr(), v_ptr, qo, ko, qw, kw, pos, inv, kp, vp, ks, vs, slots_ptr,
+            q_st, q_sh, k_st, k_sh, v_st, v_sh, qo_st, qo_sh, ko_st, ko_sh, p_sa, p_st, pg_sp,
+            pg_sh, pg_ss, num_pages, page, t, hq, hk, d, wdt, pos_bytes, 2 * half, axes, s0, s1,
+            s2, 1 if interleaved else 0, dt, q_eps, k_eps, scaling)
+    except struct.error as e:
+        raise ValueError(f"{name}: {e}") from None
+    _lib.call("umic_qk_norm_mrope_kv", dev, args)
+    return q_out, k_out
 
 
 def qk_norm_mrope_kv(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor | None,
@@ -287,15 +311,20 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     stride, width = _table("paged_attention", block_table, b)
     if out is None:
         out = q.new_empty((b, hq, d))
-    oa = _rows("paged_attention", "out", out, b, hq, d)
+        oa = (out.data_ptr(), hq * d, d)
+    else:
+        oa = _rows("paged_attention", "out", out, b, hq, d)
     lse = torch.empty((b, hq), dtype=torch.float32, device=dev) if return_lse else None
     # its own workspace for every call: calls on several streams, and graphs captured
     # apart, never share one
     need = _workspace_bytes(dev, b, hq, hk, d, width, page, dt)
     ws = q.new_empty((need + 1) // 2)
-    _lib.call("umic_paged_attention", dev, qa[0], qa[1], qa[2], k_pages.data_ptr(),
-              v_pages.data_ptr(), sp, sh, ss, p, page, dt, _lib.ptr(k_scale),
-              _lib.ptr(v_scale), block_table.data_ptr(), stride, width, kv_lens.data_ptr(), oa[0],
-              oa[1], oa[2], _lib.ptr(lse), b, hq, hk, d, scale, ws.data_ptr(), need)
+    args = _lib.pack_paged_attention_args(
+        qa[0], k_pages.data_ptr(), v_pages.data_ptr(),
+        0 if k_scale is None else k_scale.data_ptr(),
+        0 if v_scale is None else v_scale.data_ptr(), block_table.data_ptr(),
+        kv_lens.data_ptr(), oa[0], 0 if lse is None else lse.data_ptr(), ws.data_ptr(), qa[1],
+        qa[2], sp, sh, ss, p, page, stride, width, oa[1], oa[2], b, need, hq, hk, d, dt, scale)
+    _lib.call("umic_paged_attention", dev, args)
     stats["umic_paged_attention"] += 1
     return (out, lse) if return_lse else out
