@@ -81,16 +81,33 @@ __device__ __forceinline__ uint2 pack8_e4m3(const float (&f)[8]) {
   return make_uint2(w[0], w[1]);
 }
 
-constexpr int kThreads = 256, kBlocksPerSm = 2;
+// The sum over a row's lanes.
+template <int TPH>
+__device__ __forceinline__ float row_sum(float x, int mine) {
+  if constexpr ((TPH & (TPH - 1)) == 0) {
+#pragma unroll
+    for (int o = TPH / 2; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    return x;
+  }
+  float sum = 0.f;
+#pragma unroll
+  for (int j = 0; j < TPH; ++j) sum += __shfl_sync(0xffffffffu, x, min(mine * TPH + j, 31));
+  return sum;
+}
+
+constexpr int kThreads = 256;
+// CTAs per SM: what their registers allow (a write without norm and rotation needs half).
+constexpr int blocks_per_sm(bool work) { return work ? 2 : 3; }
 constexpr int kDepth = 4;  // row groups of a warp under way, 1 KB each
 
-template <int TPH, bool kE4m3>
-__global__ void __launch_bounds__(kThreads, kBlocksPerSm) mrope_kernel(MropeArgs a) {
+// TPH lanes hold a row; kWork: something is normed or rotated.
+template <int TPH, bool kE4m3, bool kWork>
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(kWork)) mrope_kernel(MropeArgs a) {
   __shared__ uint4 s_rows[kThreads / 32][kDepth][2][32];  // read by the lane that copied
   allow_dependent_launch();
   wait_prerequisite();
-  constexpr int kRows = 32 / TPH;     // rows of a group
-  constexpr int kShare = 8 / kRows;   // angles a lane makes (TPH >= 4, so at least one)
+  constexpr int kRows = 32 / TPH;                   // rows of a group
+  constexpr int kShare = (8 + kRows - 1) / kRows;   // angles a lane makes
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % TPH, mine = lane / TPH;
   const unsigned worker = blockIdx.x * (kThreads / 32) + warp;
   const int stride = gridDim.x * (kThreads / 32) / a.shares;  // tokens from one to the next
@@ -103,9 +120,10 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) mrope_kernel(MropeArgs
   if (g0 >= g1) return;
 
   const int turned = a.half / 8;  // lanes of a row whose pairs are rotated
-  const bool there = sub < a.d / 16, turns = sub < turned;
-  const int lo = turns ? sub * 8 : 2 * a.half + (sub - turned) * 16;
-  const int hi = turns ? a.half + sub * 8 : lo + 8;
+  const bool there = mine < kRows && sub < a.d / 16, turns = kWork && sub < turned;
+  // the rest of the row in two runs as well, so that lanes side by side copy side by side
+  const int lo = sub < turned ? sub * 8 : 2 * a.half + (sub - turned) * 8;
+  const int hi = lo + (sub < turned ? a.half : a.d / 2 - a.half);
 
   // ---- copies: the next group's token, place, and this lane's row of it
   const uint32_t slot0 =
@@ -152,14 +170,14 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) mrope_kernel(MropeArgs
   };
 
   // ---- this lane's share of a token's angles, and its slot, a token ahead
-  const bool angles = a.half && g0 < v_from, writes = a.k_pages && g1 > k_from;
+  const bool angles = kWork && a.half && g0 < v_from, writes = a.k_pages && g1 > k_from;
   double freq[kShare], pos[kShare];
   int64_t pos_at[kShare];
 #pragma unroll
   for (int x = 0; x < kShare; ++x) {
     freq[x] = pos[x] = 0.;
     pos_at[x] = 0;
-    const int i = min(sub * 8 + mine * kShare + x, a.half - 1);
+    const int i = min(sub * 8 + min(mine * kShare + x, 7), a.half - 1);
     if (angles) {
       freq[x] = static_cast<double>(a.inv_freq[i]) * 0.15915494309189533577;
       pos_at[x] = axis_of(a, i) * a.p_sa;
@@ -179,8 +197,9 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) mrope_kernel(MropeArgs
 #pragma unroll 1
   for (int t = first; t < a.tokens; t += stride) {
     float mc[kShare], ms[kShare];
+    if constexpr (kWork)
 #pragma unroll
-    for (int x = 0; x < kShare; ++x) turn(pos[x], freq[x], a.scaling, &mc[x], &ms[x]);
+      for (int x = 0; x < kShare; ++x) turn(pos[x], freq[x], a.scaling, &mc[x], &ms[x]);
     int64_t page_at = -1;  // where the token's K and V go; -1: nowhere
     if (writes && slot >= 0 && slot < a.num_slots) {
       const int page = slot / a.page_size;
@@ -203,32 +222,44 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) mrope_kernel(MropeArgs
              (e4m3 ? 1 : 2);
       dst_step *= e4m3 ? kRows : 2 * kRows;
       const int heads = !there || (paged && page_at < 0) ? 0 : kind ? a.hk : a.hq;  // written
-      const void* wt = kind ? a.kw : a.qw;
+      const void* wt = !kWork ? nullptr : kind ? a.kw : a.qw;
       const float eps = kind ? a.k_eps : a.q_eps;
       // x' = x xc - y ys, y' = y yc + x xs; lanes past the rotated ones: x xc, y yc
       float xc[8], ys[8], yc[8], xs[8];
+      if constexpr (kWork) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) xc[i] = yc[i] = 1.f;
-      if (wt && there) {
-        load_w8(wt, a.w_dtype, lo, xc);
-        load_w8(wt, a.w_dtype, hi, yc);
-      }
+        for (int i = 0; i < 8; ++i) xc[i] = yc[i] = 1.f;
+        if (wt && there) {
+          load_w8(wt, a.w_dtype, lo, xc);
+          load_w8(wt, a.w_dtype, hi, yc);
+        }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int src = i / kShare * TPH + sub;
-        const float c = __shfl_sync(0xffffffffu, mc[i % kShare], src);
-        const float s = __shfl_sync(0xffffffffu, ms[i % kShare], src);
-        ys[i] = yc[i] * s;
-        xs[i] = xc[i] * s;
-        if (turns) {
-          xc[i] *= c;
-          yc[i] *= c;
+        for (int i = 0; i < 8; ++i) {
+          const int src = min(i / kShare * TPH + sub, 31);
+          const float c = __shfl_sync(0xffffffffu, mc[i % kShare], src);
+          const float s = __shfl_sync(0xffffffffu, ms[i % kShare], src);
+          ys[i] = yc[i] * s;
+          xs[i] = xc[i] * s;
+          if (turns) {
+            xc[i] *= c;
+            yc[i] *= c;
+          }
         }
       }
 #pragma unroll 1
       for (int left = end - begin; left > 0; --left) {
         uint4 xv, yv;
         take(xv, yv);
+        if constexpr (!kWork && !kE4m3) {  // as it is
+          if (row < heads) {
+            st_vec(dst + 2 * lo, xv);
+            st_vec(dst + 2 * hi, yv);
+          }
+          dst += dst_step;
+          row += kRows;
+          give();
+          continue;
+        }
         float x[8], y[8];
         unpack8(xv, x);
         unpack8(yv, y);
@@ -238,8 +269,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) mrope_kernel(MropeArgs
 #pragma unroll
           for (int i = 0; i < 8; ++i) ss += x[i] * x[i] + y[i] * y[i];
           if (!there || row >= (kind ? a.hk : a.hq)) ss = 0.f;  // pieces not copied
-#pragma unroll
-          for (int o = TPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          ss = row_sum<TPH>(ss, mine);
           f = rsqrtf(ss * inv_d + eps);
         }
         if (e4m3 && a.k_scale && row < a.hk) f /= __ldg(a.k_scale + row);
@@ -250,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) mrope_kernel(MropeArgs
             y[i] = y[i] * yc[i] + x[i] * xs[i];
             x[i] = u;
           }
-        } else {
+        } else if (kWork) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             x[i] *= xc[i];
@@ -313,11 +343,16 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) mrope_kernel(MropeArgs
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-template <int TPH>
-void launch(const MropeArgs& a, int64_t blocks, cudaStream_t st) {
+template <int TPH, bool kE4m3>
+void launch_work(const MropeArgs& a, bool work, int64_t blocks, cudaStream_t st) {
   const dim3 grid(static_cast<unsigned>(blocks));
-  if (a.e4m3) launch_pdl(mrope_kernel<TPH, true>, grid, dim3(kThreads), 0, st, a);
-  else launch_pdl(mrope_kernel<TPH, false>, grid, dim3(kThreads), 0, st, a);
+  if (work) launch_pdl(mrope_kernel<TPH, kE4m3, true>, grid, dim3(kThreads), 0, st, a);
+  else launch_pdl(mrope_kernel<TPH, kE4m3, false>, grid, dim3(kThreads), 0, st, a);
+}
+template <int TPH>
+void launch(const MropeArgs& a, bool work, int64_t blocks, cudaStream_t st) {
+  if (a.e4m3) launch_work<TPH, true>(a, work, blocks, st);
+  else launch_work<TPH, false>(a, work, blocks, st);
 }
 
 }  // namespace
@@ -414,7 +449,12 @@ extern "C" int umic_qk_norm_mrope_kv(const umic_mrope_args* args, void* stream) 
   a.q_eps = q_eps;
   a.k_eps = k_eps;
   a.scaling = scaling;
-  const int tph = head_dim <= 64 ? 4 : head_dim <= 128 ? 8 : 16, at_once = 32 / tph;
+  // lanes of a row: a power of two, but for the 5 and 6 that head_dim 80 and 96 fill
+  const int tph = head_dim <= 64 ? 4 : head_dim == 80 ? 5 : head_dim == 96 ? 6
+                  : head_dim <= 128 ? 8 : 16;
+  const int at_once = 32 / tph;
+  const bool work = rotary_dim > 0 || q_weight || k_weight;
+  const int per_sm = blocks_per_sm(work);
   const int64_t groups = (static_cast<int64_t>(hq) + at_once - 1) / at_once +
                          (static_cast<int64_t>(hk) + at_once - 1) / at_once * (k_pages ? 2 : 1);
   if (groups > (1 << 20))
@@ -422,7 +462,7 @@ extern "C" int umic_qk_norm_mrope_kv(const umic_mrope_args* args, void* stream) 
   // A token's row groups go to one warp or are shared by several: the fewest rounds of
   // groups, with two more for a token's angles and start, that the GPU's resident warps
   // need for all tokens.
-  const int64_t warps = static_cast<int64_t>(sm_count()) * kBlocksPerSm * (kThreads / 32);
+  const int64_t warps = static_cast<int64_t>(sm_count()) * per_sm * (kThreads / 32);
   int64_t best = INT64_MAX;
   for (int64_t per = groups; per >= 1; per = per > 16 ? per / 2 : per - 1) {
     const int64_t shares = (groups + per - 1) / per;
@@ -436,11 +476,13 @@ extern "C" int umic_qk_norm_mrope_kv(const umic_mrope_args* args, void* stream) 
   const int64_t wanted = (tokens * a.shares + kThreads / 32 - 1) / (kThreads / 32);
   // at least a token's shares
   const int64_t blocks =
-      std::max<int64_t>(std::min<int64_t>(wanted, sm_count() * kBlocksPerSm),
+      std::max<int64_t>(std::min<int64_t>(wanted, sm_count() * per_sm),
                         (a.shares + kThreads / 32 - 1) / (kThreads / 32));
   cudaStream_t st = as_stream(stream);
-  if (tph == 4) launch<4>(a, blocks, st);
-  else if (tph == 8) launch<8>(a, blocks, st);
-  else launch<16>(a, blocks, st);
+  if (tph == 4) launch<4>(a, work, blocks, st);
+  else if (tph == 5) launch<5>(a, work, blocks, st);
+  else if (tph == 6) launch<6>(a, work, blocks, st);
+  else if (tph == 8) launch<8>(a, work, blocks, st);
+  else launch<16>(a, work, blocks, st);
   return launch_status(me);
 }
