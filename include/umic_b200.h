@@ -243,10 +243,10 @@ UMIC_API int umic_paged_plan(const int32_t* kv_lens, const int32_t* new_tokens,
 /* Attention input of ragged tokens in one pass: per-head RMSNorm (NULL weight = none),
  * rotate-half RoPE with several position axes, and the write of K and V into pages.
  * q [tokens, hq, head_dim] through (q_st, q_sh), k and v with hk heads; q_out (which
- * may be q itself) gets the rotated q. With k_pages, K and V of token t are written at
+ * may be q itself, with its strides, but not lie across it otherwise) gets the rotated q. With k_pages, K and V of token t are written at
  * slots[t] (-1: not written; other slots outside the pool set UMIC_DEVERR_BAD_PAGE and
  * are not written; two tokens must not share a slot), rounded once to cache_dtype (e4m3
- * saturates at +-448); without, the rotated k goes to k_out (which may be k) and v is
+ * saturates at +-448; scales are normal positive numbers); without, the rotated k goes to k_out (which may be k) and v is
  * not touched. The angle of pair i, which holds elements i and i + rotary_dim / 2, is
  * positions[axis(i), t] * inv_freq[i], computed in 64 bits: axis(i) = the section of
  * (s0, s1, s2) that i falls in, or with interleaved != 0 (t h w t h w ... t t) axis
@@ -284,7 +284,8 @@ UMIC_API int umic_qk_norm_mrope_kv(const umic_mrope_args* args, void* stream);
  * past max_pages * page_size is cut there; both set UMIC_DEVERR_BAD_PAGE. What lies
  * behind a request's length in its last page is never used. head_dim 64, 80, 96, 128 or
  * 256, hq a multiple of hkv, page_size a multiple of 16, 16-byte aligned bases and
- * strides. The lengths are read on the device: one captured graph serves every length.
+ * strides; the tiles of 16 tokens that the table's rows allow, times batch and KV heads
+ * (groups of more than 8 query heads count once for each 8), below 2^30. The lengths are read on the device: one captured graph serves every length.
  * workspace: umic_paged_attention_workspace_bytes() bytes, 16-byte aligned, contents
  * irrelevant before and after; calls that may overlap need one each.
  * Replaces the SDPA call of the decode step (graph.py:76-99), for rows of different

@@ -134,6 +134,8 @@ def _mrope(q=F, q_st=512, hq=4, k=F, k_st=256, v=F, hk=2, k_out=None, w=0, posit
     (dict(tokens=1 << 31), 2, "too many"), (dict(q=None), 1, "null"), (dict(k=None), 1, "null"),
     (dict(positions=None), 1, "null"), (dict(v=None), 1, "null"), (dict(slots=None), 1, "null"),
     (dict(kp=None), 1, "null"), (dict(q_st=516), 3, "alignment"),
+    (dict(pg=(8192, 64, 128)), 1, "overlap"),
+    (dict(pg=(8192, 2048, 0)), 1, "overlap"), (dict(pg=(0, 2048, 128)), 1, "overlap"),
     (dict(k=ctypes.c_void_p(4104)), 3, "alignment"), (dict(pg=(8192, 2048, 132)), 3, "alignment"),
     (dict(dt=2, pg=(8192, 2048, 136)), 3, "alignment")])
 def test_input_refusals(kw, code, text):
@@ -180,7 +182,8 @@ def test_structs_match_the_header():
     (dict(page=24), 2, "page_size 24"), (dict(num=1 << 27), 2, "2^31"),
     (dict(width=1 << 27), 2, "2^31"), (dict(batch=1 << 30), 2, "2^31"), (dict(q=None), 1, "null"),
     (dict(lens=None), 1, "null"), (dict(table=None), 1, "null"), (dict(out=None), 1, "null"),
-    (dict(q_sb=516), 3, "alignment"), (dict(pg=(8192, 2052, 128)), 3, "alignment"),
+    (dict(q_sb=516), 3, "alignment"), (dict(d=256), 1, "overlap"),
+    (dict(batch=1 << 14, num=1 << 20, width=1 << 16), 2, "2^30"), (dict(pg=(8192, 2052, 128)), 3, "alignment"),
     (dict(dt=2, pg=(8192, 2056, 128)), 3, "alignment"),
     (dict(out=ctypes.c_void_p(4098)), 3, "alignment"), (dict(ws=None), 1, "workspace"),
     (dict(ws_bytes=4), 1, "workspace"), (dict(ws=ctypes.c_void_p(4100)), 1, "workspace")])

@@ -258,6 +258,37 @@ def test_input_in_place_and_expanded_positions(cuda):
         assert torch.equal(x, y) and torch.equal(x, z)
 
 
+def test_input_far_positions(cuda):
+    """Positions up to 2^31: the angle keeps 64 bits' accuracy (2^-52 of itself, half a step
+    each for the product here and in the oracle, and one for the constant)."""
+    g = _gen(31)
+    x = torch.randn(64, 4, 128, generator=g).to(torch.bfloat16).to(cuda)
+    pos = torch.randint(1 << 30, (1 << 31) - 1, (2, 64), generator=g)
+    inv = (1e4 ** (-torch.arange(64) / 64)).to(cuda)
+    for p in (pos.to(cuda), pos.int().to(cuda)):
+        got, _ = qk_norm_mrope_kv(x, x[:, :1], None, p, inv, (20, 44), q_weight=None)
+        y, mag = oracle.norm_mrope(x, None, 0.0, pos, inv, (20, 44), False)
+        bound = _bound(y, mag, ROUNDINGS, False) + mag * 2.0 ** 31 * 2.0 ** -51
+        assert bool(((got.cpu().double() - y).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("tokens", [2367, 2368, 2369, 9000])
+def test_input_every_token_once(cuda, tokens):
+    """More and fewer tokens than resident warps, with one head and with many: every row is
+    written, and only rows that a slot names."""
+    for hk, d in ((1, 32), (9, 80)):
+        k = torch.full((tokens, hk, d), 2.0, dtype=torch.bfloat16, device=cuda)
+        pages = tokens // 16 + 2
+        kp = torch.zeros(pages, hk, 16, d, dtype=torch.bfloat16, device=cuda)
+        vp = torch.zeros_like(kp)
+        slots = torch.arange(tokens, dtype=torch.int32, device=cuda) + 5
+        paged_kv_append(kp, vp, k, -k, slots)
+        flat = kp.transpose(1, 2).reshape(-1, hk, d)
+        assert bool((flat[5:5 + tokens] == 2).all())
+        assert bool((flat[:5] == 0).all()) and bool((flat[5 + tokens:] == 0).all())
+        assert torch.equal(vp, -kp)
+
+
 def test_input_special_values(cuda):
     """e4m3 saturates at 448 and keeps NaN; -1 and bad slots write nothing."""
     kp, vp, ks, vs = _pool(1, 3, 1, 16, 16, True, cuda)
@@ -535,6 +566,8 @@ def test_input_wrapper_refusals(cuda):
             (TypeError, dict(k_pages=e, v_pages=e, k_scale=z(2))),
             (TypeError, dict(k_pages=e.view(torch.float8_e5m2), v_pages=e.view(torch.float8_e5m2))),
             (ValueError, dict(q_weight=z(65))), (ValueError, dict(q_out=z(3, 5, 64))),
+            (RuntimeError, dict(q_out=z(3, 1, 64).expand(3, 4, 64))),
+            (ValueError, dict(sections=(1 << 40, 10, 10))), (ValueError, dict(k_out=z(3, 2, 64))),
             (TypeError, dict(q_weight=z(64), k_weight=z(64, dtype=torch.float32)))]:
         with pytest.raises(error):
             qk_norm_mrope_kv(**{**good, **change})
@@ -554,6 +587,7 @@ def test_attend_wrapper_refusals(cuda):
             (ValueError, dict(block_table=z(2, 2, dtype=torch.int64))),
             (TypeError, dict(kv_lens=z(2, dtype=torch.int64))),
             (ValueError, dict(kv_lens=z(3, dtype=i32))), (ValueError, dict(out=z(2, 5, 64))),
+            (RuntimeError, dict(out=z(2, 1, 64).expand(2, 4, 64))),
             (RuntimeError, dict(k_pages=pages, v_pages=pages)),
             (ValueError, dict(v_pages=z(4, 2, 16, 64).transpose(1, 2)))]:
         with pytest.raises(error):

@@ -395,7 +395,7 @@ extern "C" int umic_qk_norm_mrope_kv(const umic_mrope_args* args, void* stream) 
   if (k_pages && (num_pages <= 0 || page_size <= 0 || page_size > 0x7fffffffLL / num_pages))
     return fail(UMIC_ERR_UNSUPPORTED, "%s: num_pages %lld x page_size %lld must stay below 2^31",
                 me, (long long)num_pages, (long long)page_size);
-  if (tokens > 0x7fffffffLL)
+  if (tokens > 0x7fff0000LL)
     return fail(UMIC_ERR_UNSUPPORTED, "%s: too many tokens (%lld)", me, (long long)tokens);
   if (tokens == 0) return UMIC_OK;
   if (!k || (hq > 0 && (!q || !q_out)) || (rotary_dim > 0 && (!positions || !inv_freq)) ||
@@ -411,6 +411,15 @@ extern "C" int umic_qk_norm_mrope_kv(const umic_mrope_args* args, void* stream) 
                : aligned16(k_out) && ko_st % 8 == 0 && ko_sh % 8 == 0);
   if (!q_al || !kv_al || (q_weight && !aligned16(q_weight)) || (k_weight && !aligned16(k_weight)))
     return fail(UMIC_ERR_ALIGNMENT, "%s: 16-byte alignment of bases / strides", me);
+  // rows written: apart from one another
+  auto apart = [&](int64_t st, int64_t sh, int32_t heads) {
+    return (heads <= 1 || sh >= head_dim) && (tokens <= 1 || st >= head_dim);
+  };
+  if ((hq > 0 && !apart(qo_st, qo_sh, hq)) ||
+      (k_pages ? (hk > 1 && pg_sh < head_dim) || pg_ss < head_dim ||
+                     (num_pages > 1 && pg_sp < head_dim)
+               : !apart(ko_st, ko_sh, hk)))
+    return fail(UMIC_ERR_INVALID_ARG, "%s: output rows overlap", me);
   uint32_t* err = device_error_word();
   if (!err) return fail(UMIC_ERR_DEVICE, "%s: no device error word", me);
   MropeArgs a{};

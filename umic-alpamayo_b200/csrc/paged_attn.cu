@@ -326,6 +326,7 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
   __shared__ Split s_split[kWarps];
 
   allow_dependent_launch();
+  if (threadIdx.x < kWarps) s_begin[threadIdx.x] = make_int4(0, 0, 0, 0);
   wait_prerequisite();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int hcs = a.hkv * a.chunks;  // segments per request
@@ -351,9 +352,8 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
     for (int w = 0; w < kWarps && first_worker + w < workers; ++w) {
       int at = line.begin(first_worker + w) - upto * hcs;
       if (at < 0 || at >= mine * hcs) continue;
-      int len = first_len;
-      for (int b = b0;; len = clamped_len(a, ++b)) {
-        const int tiles = tiles_of(len);
+      for (int b = b0; b < b1; ++b) {
+        const int len = b == b0 ? first_len : clamped_len(a, b), tiles = tiles_of(len);
         if (at < tiles * hcs) {
           s_begin[w] = make_int4(b, at / tiles, at % tiles, len);
           break;
@@ -490,8 +490,7 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
             llen = other_len;
             entries_first = other_entries;
             if (llen == 0) {  // the requests behind an empty one are looked up in turn
-              do llen = clamped_len(a, ++lb);
-              while (llen == 0);
+              while (llen == 0 && lb + 1 < a.batch) llen = clamped_len(a, ++lb);
               entries_first = entry(lb, lane);
             }
             ltiles = tiles_of(llen);
@@ -1103,9 +1102,9 @@ extern "C" int umic_paged_attention(const umic_paged_attention_args* args, void*
                 me);
   // tiles of every segment, had every request the longest row, count in 32 bits
   const int64_t segments = static_cast<int64_t>(batch) * hkv * ((hq / hkv + 7) / 8);
-  if (segments > 0x7fffffffLL / std::max<int64_t>(1, max_pages * page_size / kSub))
+  if (segments > 0x3fffffffLL / std::max<int64_t>(1, max_pages * page_size / kSub))
     return fail(UMIC_ERR_UNSUPPORTED,
-                "%s: batch * KV heads * max_pages * page_size / 16 must stay below 2^31", me);
+                "%s: batch * KV heads * max_pages * page_size / 16 must stay below 2^30", me);
   if (batch == 0) return UMIC_OK;
   if (!q || !k_pages || !v_pages || !kv_lens || !out || (max_pages > 0 && !block_table))
     return fail(UMIC_ERR_INVALID_ARG, "%s: null pointer", me);
@@ -1113,6 +1112,8 @@ extern "C" int umic_paged_attention(const umic_paged_attention_args* args, void*
   if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out) ||
       q_sb % 8 || q_sh % 8 || o_sb % 8 || o_sh % 8 || pg_sp % pe || pg_sh % pe || pg_ss % pe)
     return fail(UMIC_ERR_ALIGNMENT, "%s: 16-byte alignment of bases / strides", me);
+  if ((hq > 1 && o_sh < head_dim) || (batch > 1 && o_sb < head_dim))
+    return fail(UMIC_ERR_INVALID_ARG, "%s: output rows overlap", me);
   const size_t need = umic_paged_attention_workspace_bytes(batch, hq, hkv, head_dim, max_pages,
                                                            page_size, cache_dtype);
   if (!workspace || !aligned16(workspace) || workspace_bytes < static_cast<int64_t>(need))
