@@ -412,8 +412,9 @@ extern "C" int umic_qk_norm_mrope_kv(const umic_mrope_args* args, void* stream) 
   if (!q_al || !kv_al || (q_weight && !aligned16(q_weight)) || (k_weight && !aligned16(k_weight)))
     return fail(UMIC_ERR_ALIGNMENT, "%s: 16-byte alignment of bases / strides", me);
   // rows written: apart from one another
-  auto apart = [&](int64_t st, int64_t sh, int32_t heads) {
-    return (heads <= 1 || sh >= head_dim) && (tokens <= 1 || st >= head_dim);
+  const int64_t n_tokens = tokens, width = head_dim;
+  auto apart = [n_tokens, width](int64_t st, int64_t sh, int32_t heads) {
+    return (heads <= 1 || sh >= width) && (n_tokens <= 1 || st >= width);
   };
   if ((hq > 0 && !apart(qo_st, qo_sh, hq)) ||
       (k_pages ? (hk > 1 && pg_sh < head_dim) || pg_ss < head_dim ||
