@@ -20,6 +20,9 @@
 // out among the row groups' lanes and handed round by shuffles, times the norm's weights,
 // when the warp comes to the q rows and to the k rows:
 //   out[i] = rstd (x[i] w[i] cos - x[i + r/2] w[i + r/2] sin), and so on.
+// Measured: 24800 tokens of 32 + 8 + 8 heads x 128 into e4m3 pages 107 us (0.80 of measured
+// HBM, issue slots 0.61 busy), 3100 into bf16 pages 17.7 us, 16384 x (16 + 16) x 80 without
+// norm or cache 38 us (0.67), 6200 tokens appended as they are 10 us (0.78), 8 tokens 3.2 us.
 #include <cuda_fp8.h>
 
 #include <algorithm>
