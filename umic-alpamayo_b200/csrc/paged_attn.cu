@@ -16,7 +16,7 @@
 //   S^T = K Q^T    mma.sync m16n8k16, tokens as rows: the 8 columns are query heads, so a
 //                  group of up to 8 heads costs one instruction per 16 dims (tcgen05 wants
 //                  64 or 128 rows per operand and a block-wide hand-over of each tile;
-//                  here the tensor pipe is busy a few per cent of the time either way)
+//                  here the tensor pipe is busy 10 to 16 per cent of the time)
 //   m, l, P        running maximum and sum of each head, fp32, base 2
 //   O^T += V^T P   V through transposing ldmatrix, P transposed in registers
 // P is fp32 split into a bf16 value and its bf16 remainder (two products, weights held to
