@@ -470,6 +470,27 @@ def test_attend_extreme_scores(cuda):
     assert bool(out2[1, 2:, :5].isfinite().all())
 
 
+@pytest.mark.parametrize("d", [64, 80, 128])
+@pytest.mark.parametrize("code", [0x7f, 0xff])
+def test_attend_e4m3_nan_and_largest(cuda, d, code):
+    """NaN of either sign in a valid token: in V it makes its dim NaN for the heads of its
+    KV head, in K their whole rows, whatever the sign of q; +-448 are values like others."""
+    c = _attend_case(13, [50, 20, 700], 8, 2, d, 16, True, cuda)
+    q, kp, vp, table, lens, scale, ks, vs = c
+    kp.view(torch.uint8)[table[0, 0], :, 3, ::7] = 0x7e
+    vp.view(torch.uint8)[table[0, 1], :, 2, ::5] = 0xfe
+    _check_attend(cuda, *c)
+    args = (table.to(cuda), lens.to(cuda), scale)
+    clean = paged_attention(q, kp, vp, *args, k_scale=ks, v_scale=vs)
+    vp.view(torch.uint8)[table[0, 2], 1, 1, 9] = code
+    kp.view(torch.uint8)[table[2, 30], 0, 5, 11] = code
+    out, lse = paged_attention(q, kp, vp, *args, k_scale=ks, v_scale=vs, return_lse=True)
+    assert bool(out[0, 4:, 9].isnan().all()) and bool(out[2, :4].isnan().all())
+    assert bool(lse[2, :4].isnan().all()) and bool(lse[0].isfinite().all())
+    out[0, 4:, 9], out[2, :4] = clean[0, 4:, 9], clean[2, :4]
+    assert torch.equal(out, clean)
+
+
 def test_attend_strided_q_and_out(cuda):
     """q as a slice of a packed projection, out into a wider buffer left alone around it."""
     c = _attend_case(12, [33, 80], 8, 2, 128, 16, False, cuda)
@@ -588,6 +609,7 @@ def test_attend_wrapper_refusals(cuda):
             (TypeError, dict(kv_lens=z(2, dtype=torch.int64))),
             (ValueError, dict(kv_lens=z(3, dtype=i32))), (ValueError, dict(out=z(2, 5, 64))),
             (RuntimeError, dict(out=z(2, 1, 64).expand(2, 4, 64))),
+            (ValueError, dict(scale="0.1")),
             (RuntimeError, dict(k_pages=pages, v_pages=pages)),
             (ValueError, dict(v_pages=z(4, 2, 16, 64).transpose(1, 2)))]:
         with pytest.raises(error):

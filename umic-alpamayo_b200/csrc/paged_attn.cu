@@ -208,8 +208,8 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 // Four e4m3 values as fp16 pairs (bytes 0, 2 and bytes 1, 3), times kWide, exactly. The
 // seven bits below the sign, put three places higher in fp16, are the value times 2^-8,
 // subnormals included; the product with 2^8 kWide has 4 + 6 bits, is normal, and sends the
-// NaN code (which the shift makes 480 * 2^-8) over the largest fp16 to infinity, so that a
-// NaN in K or V still reaches its rows. Nine instructions, five of them on the ALU pipe,
+// NaN code (which the shift makes 480 * 2^-8) over the largest fp16 to infinity, which the
+// scores and the output turn into NaN again. Nine instructions, five of them on the ALU pipe,
 // which the conversion instruction would fill.
 constexpr float kWide = 140.f;
 __device__ __forceinline__ void widen4(uint32_t r, uint32_t& even, uint32_t& odd) {
@@ -255,12 +255,14 @@ struct Rows {
     __nv_bfloat16* base = a.out + b * a.o_sb + static_cast<int64_t>(head0(a, hc)) * a.o_sh;
     if constexpr (kE4m3) {  // rows g and g + 8 are dims 2g and 2g + 1
       const int h = nt * 8 + 2 * c;
+      // infinite only by a NaN in V: NaN again
+      auto norm = [](float x, float inv) { return fmaf(x, 0.f, x * inv); };
       if (h < n)
         *reinterpret_cast<uint32_t*>(base + h * a.o_sh + md * 16 + 2 * g) =
-            pack_bf16(o.x * inv0, o.z * inv0);
+            pack_bf16(norm(o.x, inv0), norm(o.z, inv0));
       if (h + 1 < n)
         *reinterpret_cast<uint32_t*>(base + (h + 1) * a.o_sh + md * 16 + 2 * g) =
-            pack_bf16(o.y * inv1, o.w * inv1);
+            pack_bf16(norm(o.y, inv1), norm(o.w, inv1));
     } else {
       const uint32_t lo = transpose8x8(pack_bf16(o.x * inv0, o.y * inv1));
       const uint32_t hi = transpose8x8(pack_bf16(o.z * inv0, o.w * inv1));
@@ -634,10 +636,13 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
 #pragma unroll
       for (int u = 0; u < MT; ++u) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          x[u][j] = (MT == 2 ? s[nt][2 * u][j] + s[nt][2 * u + 1][j]
-                             : (s[nt][0][j] + s[nt][1][j]) + (s[nt][2][j] + s[nt][3][j])) *
-                    fac[nt][j & 1];
+        for (int j = 0; j < 4; ++j) {
+          const float sum = MT == 2 ? s[nt][2 * u][j] + s[nt][2 * u + 1][j]
+                                    : (s[nt][0][j] + s[nt][1][j]) + (s[nt][2][j] + s[nt][3][j]);
+          x[u][j] = sum * fac[nt][j & 1];
+          // infinite only by a NaN in K (widen4): a NaN score, not a weight of 0
+          if constexpr (kE4m3) x[u][j] = fmaf(sum, 0.f, x[u][j]);
+        }
         const int rows = rows_of >> (8 * u) & 255;
         if (rows < kSub) {
           if (g >= rows) x[u][0] = x[u][1] = -INFINITY;

@@ -319,12 +319,16 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     # apart, never share one
     need = _workspace_bytes(dev, b, hq, hk, d, width, page, dt)
     ws = q.new_empty((need + 1) // 2)
-    args = _lib.pack_paged_attention_args(
-        qa[0], k_pages.data_ptr(), v_pages.data_ptr(),
-        0 if k_scale is None else k_scale.data_ptr(),
-        0 if v_scale is None else v_scale.data_ptr(), block_table.data_ptr(),
-        kv_lens.data_ptr(), oa[0], 0 if lse is None else lse.data_ptr(), ws.data_ptr(), qa[1],
-        qa[2], sp, sh, ss, p, page, stride, width, oa[1], oa[2], b, need, hq, hk, d, dt, scale)
+    try:
+        args = _lib.pack_paged_attention_args(
+            qa[0], k_pages.data_ptr(), v_pages.data_ptr(),
+            0 if k_scale is None else k_scale.data_ptr(),
+            0 if v_scale is None else v_scale.data_ptr(), block_table.data_ptr(),
+            kv_lens.data_ptr(), oa[0], 0 if lse is None else lse.data_ptr(), ws.data_ptr(),
+            qa[1], qa[2], sp, sh, ss, p, page, stride, width, oa[1], oa[2], b, need, hq, hk, d,
+            dt, scale)
+    except struct.error as e:
+        raise ValueError(f"paged_attention: {e}") from None
     _lib.call("umic_paged_attention", dev, args)
     stats["umic_paged_attention"] += 1
     return (out, lse) if return_lse else out
