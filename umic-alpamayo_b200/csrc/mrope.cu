@@ -13,10 +13,10 @@
 // HBM bounds it: every row is read and written once, 24 KB for a token of 32 + 8 + 8 heads,
 // and the issue slots run close behind, so the work per row is kept small. A group of TPH
 // lanes owns a head row, 16 elements a lane: 8 of the first half and their rotary partners,
-// so the rotation needs no exchange and the norm log2(TPH) shuffles. A warp walks over
-// tokens and in each over row groups (32 / TPH rows of one kind: q, k or v), all of them or
-// a share; each lane copies its own pieces of the next kDepth groups, across tokens, into
-// shared memory with asynchronous loads. A token's angles are made once per warp, shared
+// so the rotation needs no exchange and the norm log2(TPH) shuffles. The row groups (32 / TPH
+// rows of one kind: q, k or v) of all tokens form one line, and every resident warp walks
+// over an equal run of it; each lane copies its own pieces of the next kDepth groups, across
+// tokens, into shared memory with asynchronous loads. A token's angles are made once per warp, shared
 // out among the row groups' lanes and handed round by shuffles, times the norm's weights,
 // when the warp comes to the q rows and to the k rows:
 //   out[i] = rstd (x[i] w[i] cos - x[i + r/2] w[i + r/2] sin), and so on.
@@ -43,7 +43,8 @@ struct MropeArgs {
   int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, qo_st, qo_sh, ko_st, ko_sh;
   int64_t p_sa, p_st, pg_sp, pg_sh, pg_ss, num_slots;
   int32_t page_size, tokens, hq, hk, d, half;
-  int32_t shares, groups;  // warps of a token, row groups of each
+  int64_t run;      // row groups of a warp,
+  int32_t longer;   // one more for the first so many
   int32_t sec[3], axes, interleaved, pos64, w_dtype, e4m3;
   float q_eps, k_eps, scaling;
 };
@@ -112,15 +113,15 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kWork)) mrope_kernel(M
   constexpr int kRows = 32 / TPH;                   // rows of a group
   constexpr int kShare = (8 + kRows - 1) / kRows;   // angles a lane makes
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % TPH, mine = lane / TPH;
-  const unsigned worker = blockIdx.x * (kThreads / 32) + warp;
-  const int stride = gridDim.x * (kThreads / 32) / a.shares;  // tokens from one to the next
-  const int first = worker / a.shares;
-  if (first >= stride || first >= a.tokens) return;
-  const int g0 = worker % a.shares * a.groups;
+  const int64_t worker = blockIdx.x * (kThreads / 32) + warp;
   const int k_from = (a.hq + kRows - 1) / kRows, v_from = k_from + (a.hk + kRows - 1) / kRows;
   const int all = a.k_pages ? 2 * v_from - k_from : v_from;  // row groups, q before k before v
-  const int g1 = min(all, g0 + a.groups);
-  if (g0 >= g1) return;
+  const int64_t begin_at = worker * a.run + min(worker, static_cast<int64_t>(a.longer));
+  int run = static_cast<int>(a.run + (worker < a.longer));  // still to do
+  if (run <= 0) return;
+  const int first = static_cast<int>(
+      begin_at >> 32 ? begin_at / all : static_cast<uint32_t>(begin_at) / static_cast<uint32_t>(all));
+  const int first_group = static_cast<int>(begin_at - static_cast<int64_t>(first) * all);
 
   const int turned = a.half / 8;  // lanes of a row whose pairs are rotated
   const bool there = mine < kRows && sub < a.d / 16, turns = kWork && sub < turned;
@@ -131,15 +132,16 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kWork)) mrope_kernel(M
   // ---- copies: the next group's token, place, and this lane's row of it
   const uint32_t slot0 =
       static_cast<uint32_t>(__cvta_generic_to_shared(&s_rows[warp][0][0][lane]));
-  int ct = first, cg = g0, cg_end = g0, crow = 0, cheads = 0;
+  int ct = first, cg = first_group, cg_end = first_group, crow = 0, cheads = 0, to_copy = run;
   const __nv_bfloat16* csrc = nullptr;
   int64_t cstep = 0;
   auto copy = [&](int stage) {
-    if (ct < a.tokens) {
+    if (to_copy > 0) {
+      --to_copy;
       if (cg == cg_end) {  // a kind of rows begins
         const int from = cg < k_from ? 0 : cg < v_from ? k_from : v_from;
         const int64_t sh = cg < k_from ? a.q_sh : cg < v_from ? a.k_sh : a.v_sh;
-        cg_end = min(g1, cg < k_from ? k_from : cg < v_from ? v_from : all);
+        cg_end = cg < k_from ? k_from : cg < v_from ? v_from : all;
         cheads = !there ? 0 : cg < k_from ? a.hq : a.hk;
         crow = (cg - from) * kRows + mine;
         csrc = (cg < k_from ? a.q + ct * a.q_st : cg < v_from ? a.k + ct * a.k_st
@@ -152,9 +154,9 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kWork)) mrope_kernel(M
       }
       csrc += cstep;
       crow += kRows;
-      if (++cg == g1) {
-        cg = cg_end = g0;
-        ct += stride;
+      if (++cg == all) {
+        cg = cg_end = 0;
+        ++ct;
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -173,7 +175,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kWork)) mrope_kernel(M
   };
 
   // ---- this lane's share of a token's angles, and its slot, a token ahead
-  const bool angles = kWork && a.half && g0 < v_from, writes = a.k_pages && g1 > k_from;
+  const bool angles = kWork && a.half, writes = a.k_pages;
   double freq[kShare], pos[kShare];
   int64_t pos_at[kShare];
 #pragma unroll
@@ -198,9 +200,11 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kWork)) mrope_kernel(M
   const float inv_d = 1.f / static_cast<float>(a.d);
 
 #pragma unroll 1
-  for (int t = first; t < a.tokens; t += stride) {
+  for (int t = first, g0 = first_group; run > 0; ++t, g0 = 0) {
+    const int g1 = min(all, g0 + run);  // this token's groups
+    run -= g1 - g0;
     float mc[kShare], ms[kShare];
-    if constexpr (kWork)
+    if (kWork && g0 < v_from)
 #pragma unroll
       for (int x = 0; x < kShare; ++x) turn(pos[x], freq[x], a.scaling, &mc[x], &ms[x]);
     int64_t page_at = -1;  // where the token's K and V go; -1: nowhere
@@ -210,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kWork)) mrope_kernel(M
     } else if (writes && slot != -1 && lane == 0) {
       atomicOr(a.err, UMIC_DEVERR_BAD_PAGE);
     }
-    look(t + stride);
+    if (run > 0) look(t + 1);
 
 #pragma unroll 1
     for (int kind = g0 < k_from ? 0 : 1; kind < 2; ++kind) {  // q, k
@@ -472,25 +476,16 @@ extern "C" int umic_qk_norm_mrope_kv(const umic_mrope_args* args, void* stream) 
                          (static_cast<int64_t>(hk) + at_once - 1) / at_once * (k_pages ? 2 : 1);
   if (groups > (1 << 20))
     return fail(UMIC_ERR_UNSUPPORTED, "%s: too many heads (%d + %d)", me, hq, hk);
-  // A token's row groups go to one warp or are shared by several: the fewest rounds of
-  // groups, with two more for a token's angles and start, that the GPU's resident warps
-  // need for all tokens.
-  const int64_t warps = static_cast<int64_t>(sm_count()) * per_sm * (kThreads / 32);
-  int64_t best = INT64_MAX;
-  for (int64_t per = groups; per >= 1; per = per > 16 ? per / 2 : per - 1) {
-    const int64_t shares = (groups + per - 1) / per;
-    const int64_t rounds = (tokens * shares + warps - 1) / warps * (per + 2);
-    if (rounds < best) {
-      best = rounds;
-      a.groups = static_cast<int32_t>(per);
-      a.shares = static_cast<int32_t>(shares);
-    }
-  }
-  const int64_t wanted = (tokens * a.shares + kThreads / 32 - 1) / (kThreads / 32);
-  // at least a token's shares
-  const int64_t blocks =
-      std::max<int64_t>(std::min<int64_t>(wanted, sm_count() * per_sm),
-                        (a.shares + kThreads / 32 - 1) / (kThreads / 32));
+  // a group for every resident warp, more while there are more
+  const int64_t total = tokens * groups;
+  const int64_t blocks = std::min<int64_t>((total + kThreads / 32 - 1) / (kThreads / 32),
+                                           static_cast<int64_t>(sm_count()) * per_sm);
+  const int64_t warps = blocks * (kThreads / 32);
+  a.run = total / warps;
+  a.longer = static_cast<int32_t>(total % warps);
+  if (a.run >= 0x7fffffffLL)
+    return fail(UMIC_ERR_UNSUPPORTED, "%s: %lld tokens x %lld heads", me, (long long)tokens,
+                (long long)hq + hk);
   cudaStream_t st = as_stream(stream);
   if (tph == 4) launch<4>(a, work, blocks, st);
   else if (tph == 5) launch<5>(a, work, blocks, st);
