@@ -614,3 +614,18 @@ def test_attend_wrapper_refusals(cuda):
             (ValueError, dict(v_pages=z(4, 2, 16, 64).transpose(1, 2)))]:
         with pytest.raises(error):
             paged_attention(**{**good, **change})
+
+
+def test_attend_many_requests(cuda):
+    """More requests than threads of a CTA: each equals the same request in a small batch."""
+    g = _gen(77)
+    lens = torch.randint(0, 17, (20000,), generator=g)
+    kp, vp, _, _ = _pool(3, 300, 2, 16, 64, False, cuda)
+    table = torch.randint(0, 300, (20000, 1), generator=g).int().to(cuda)
+    q = torch.randn(20000, 4, 64, generator=g).to(torch.bfloat16).to(cuda)
+    lens = lens.int().to(cuda)
+    out = paged_attention(q, kp, vp, table, lens, 0.125)
+    for a in range(0, 20000, 4000):
+        s = slice(a, a + 100)
+        assert torch.equal(out[s], paged_attention(q[s], kp, vp, table[s], lens[s], 0.125))
+    assert bool((out[lens == 0] == 0).all())

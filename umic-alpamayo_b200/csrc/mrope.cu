@@ -20,9 +20,11 @@
 // out among the row groups' lanes and handed round by shuffles, times the norm's weights,
 // when the warp comes to the q rows and to the k rows:
 //   out[i] = rstd (x[i] w[i] cos - x[i + r/2] w[i + r/2] sin), and so on.
-// Measured: 24800 tokens of 32 + 8 + 8 heads x 128 into e4m3 pages 107 us (0.80 of measured
-// HBM, issue slots 0.61 busy), 3100 into bf16 pages 17.7 us, 16384 x (16 + 16) x 80 without
-// norm or cache 38 us (0.67), 6200 tokens appended as they are 10 us (0.78), 8 tokens 3.2 us.
+// Measured: 24800 tokens of 32 + 8 + 8 heads x 128 into e4m3 pages 101 us (0.85 of measured
+// HBM, issue slots 0.68 busy), 3100 into bf16 pages 14.5 us (0.80), 16384 x (16 + 16) x 80
+// without norm or cache 37.5 us (0.68), 6200 tokens appended as they are 9.7 us (0.80), 8
+// tokens 3.2 us. (Whole tokens or shares of one to a warp instead of equal runs: 108 and
+// 17.7 us for the first two.)
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -101,7 +103,7 @@ __device__ __forceinline__ float row_sum(float x, int mine) {
 
 constexpr int kThreads = 256;
 // CTAs per SM: what their registers allow (a write without norm and rotation needs half).
-constexpr int blocks_per_sm(bool work) { return work ? 2 : 3; }
+constexpr int blocks_per_sm(bool work) { return work ? 2 : 4; }
 constexpr int kDepth = 4;  // row groups of a warp under way, 1 KB each
 
 // TPH lanes hold a row; kWork: something is normed or rotated.

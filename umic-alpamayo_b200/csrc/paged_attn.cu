@@ -33,7 +33,7 @@
 // runs once, at the end, from a cold instruction cache.)
 //
 // Measured, both kernels, 32 query and 8 KV heads x 128: 32 requests of up to 32768 tokens
-// (2.2 GB) 345 us, 0.97 of measured HBM; 8 of 3164 tokens (104 MB) 26.6 us, of which 16 us
+// (2.2 GB) 346 us, 0.97 of measured HBM; 8 of 3164 tokens (104 MB) 26.6 us, of which 16 us
 // stream and 10 us are start, join and the spread of the warps' ends; 1 of 3164 12.9 us.
 // 256 requests of up to 4096 tokens in e4m3 pages, 16 and 8 heads (1.04 GB) 206 us: there
 // the widening (half of a tile's instructions) bounds it as much as HBM.
