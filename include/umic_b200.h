@@ -243,11 +243,15 @@ UMIC_API int umic_paged_plan(const int32_t* kv_lens, const int32_t* new_tokens,
 /* Attention input of ragged tokens in one pass: per-head RMSNorm (NULL weight = none),
  * rotate-half RoPE with several position axes, and the write of K and V into pages.
  * q [tokens, hq, head_dim] through (q_st, q_sh), k and v with hk heads; q_out (which
- * may be q itself, with its strides, but not lie across it otherwise) gets the rotated q. With k_pages, K and V of token t are written at
- * slots[t] (-1: not written; other slots outside the pool set UMIC_DEVERR_BAD_PAGE and
- * are not written; two tokens must not share a slot), rounded once to cache_dtype (e4m3
- * saturates at +-448; scales are normal positive numbers); without, the rotated k goes to k_out (which may be k) and v is
- * not touched. The angle of pair i, which holds elements i and i + rotary_dim / 2, is
+ * may be q itself, with its strides, but not lie across it otherwise) gets the rotated q.
+ * With k_pages, K and V of token t are written at slots[t] (-1: not written; other slots
+ * outside the pool set UMIC_DEVERR_BAD_PAGE and are not written; two tokens must not
+ * share a slot), rounded once to cache_dtype (e4m3 saturates at +-448; scales are normal
+ * positive numbers); without, the rotated k goes to k_out (which may be k) and v is not
+ * touched. Bases are 16-byte aligned, strides multiples of 16 bytes. Rows that are written
+ * lie apart: the axes of q_out, k_out and the pages may come in any order, but each steps
+ * over all that those of smaller stride span (UMIC_ERR_INVALID_ARG otherwise).
+ * The angle of pair i, which holds elements i and i + rotary_dim / 2, is
  * positions[axis(i), t] * inv_freq[i], computed in 64 bits: axis(i) = the section of
  * (s0, s1, s2) that i falls in, or with interleaved != 0 (t h w t h w ... t t) axis
  * i % axes while i < axes * s_axis, else axis 0. Sections sum to rotary_dim / 2; cos

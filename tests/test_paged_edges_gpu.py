@@ -1,0 +1,69 @@
+"""GPU tests of the paged-cache serving operators at the edges of what their documentation
+allows: layouts, the largest tables, borders of the cache's type, requests that a long walk
+of one warp covers."""
+
+import itertools
+
+import pytest
+import torch
+
+from umic_b200.kernels import paged_kv_append, qk_norm_mrope_kv
+
+pytestmark = pytest.mark.gpu
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _ordered(shape, order, dev, pad=0):
+    """Zeros of `shape` [..., D] whose leading axes lie in memory in `order`; the innermost
+    of them with `pad` unused elements behind each row."""
+    dims = [shape[a] for a in order]
+    wide = torch.zeros(*dims, shape[-1] + pad, dtype=torch.bfloat16, device=dev)[..., :shape[-1]]
+    back = [order.index(a) for a in range(len(order))]
+    return wide.permute(*back, len(order))
+
+
+# ----------------------------------------------------------------- layouts
+
+@pytest.mark.parametrize("pad", [0, 8])
+def test_input_writes_rows_in_any_order_of_axes(cuda, pad):
+    """Rotated q and k, and pages, in every order of their axes, tight or with room between
+    the rows: the bits of the plain layout."""
+    g = _gen(41)
+    t, hq, hk, d, page = 37, 6, 3, 64, 16
+    q, k, v = (torch.randn(t, h, d, generator=g).to(torch.bfloat16).to(cuda)
+               for h in (hq, hk, hk))
+    pos = torch.randint(0, 5000, (3, t), generator=g).to(cuda)
+    inv = (1e6 ** (-torch.arange(32) / 32)).to(cuda)
+    slots = torch.randperm(5 * page, generator=g)[:t].int().to(cuda)
+    args = (q, k, v, pos, inv, (12, 10, 10))
+    want_q, want_k = qk_norm_mrope_kv(q, k, None, *args[3:])
+    kp = torch.zeros(5, hk, page, d, dtype=torch.bfloat16, device=cuda)
+    vp = torch.zeros_like(kp)
+    qk_norm_mrope_kv(*args, k_pages=kp, v_pages=vp, slots=slots)
+    for order in itertools.permutations(range(2)):
+        q_out = _ordered((t, hq, d), order, cuda, pad=pad)
+        k_out = _ordered((t, hk, d), order, cuda, pad=pad)
+        qk_norm_mrope_kv(q, k, None, *args[3:], q_out=q_out, k_out=k_out)
+        assert torch.equal(q_out, want_q) and torch.equal(k_out, want_k)
+    for order in itertools.permutations(range(3)):
+        kx, vx = (_ordered(kp.shape, order, cuda, pad=pad) for _ in range(2))
+        q_out, _ = qk_norm_mrope_kv(*args, k_pages=kx, v_pages=vx, slots=slots)
+        assert torch.equal(q_out, want_q)
+        assert torch.equal(kx, kp) and torch.equal(vx, vp)
+
+
+def test_single_entries_need_no_stride(cuda):
+    """The stride of an axis of one entry is never used: one token, one head, one page."""
+    d = 64
+    g = _gen(42)
+    k = torch.randn(1, 2, d, generator=g).to(torch.bfloat16).to(cuda)
+    pages = torch.zeros(2 * 16 * d, dtype=torch.bfloat16, device=cuda)
+    kp = pages.as_strided((1, 2, 16, d), (0, 16 * d, d, 1))
+    vp = torch.zeros_like(pages).as_strided((1, 2, 16, d), (0, 16 * d, d, 1))
+    slots = torch.tensor([7], dtype=torch.int32, device=cuda)
+    paged_kv_append(kp, vp, k, -k, slots)
+    assert torch.equal(kp[0, :, 7], k[0]) and torch.equal(vp[0, :, 7], -k[0])
+    assert int((pages != 0).sum()) <= 2 * d

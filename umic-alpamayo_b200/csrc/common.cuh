@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <cstdarg>
 #include <mutex>
 #include <cstdio>
@@ -35,6 +36,26 @@ constexpr int kGemvGeneralMerge = 3;  // not a stall: the next GEMV skips its fa
 bool take_stall(int kernel, long long* limit);
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// An axis of a strided array of rows; strides in elements.
+struct Axis {
+  int64_t extent, stride;
+};
+
+// Whether rows of `width` elements lie apart: taken from the smallest stride up, an axis of
+// more than one entry steps over all that the axes before it span. (Every permutation and
+// slice of a dense array does; rows that interleave otherwise without meeting do not count.)
+template <int N>
+inline bool rows_apart(Axis (&&axes)[N], int64_t width) {
+  std::sort(axes, axes + N, [](const Axis& x, const Axis& y) { return x.stride < y.stride; });
+  __int128 span = width;
+  for (const Axis& x : axes) {
+    if (x.extent <= 1) continue;
+    if (x.stride < span) return false;
+    span += static_cast<__int128>(x.extent - 1) * x.stride;
+  }
+  return true;
+}
 
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 

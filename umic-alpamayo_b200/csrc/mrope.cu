@@ -421,14 +421,9 @@ extern "C" int umic_qk_norm_mrope_kv(const umic_mrope_args* args, void* stream) 
   if (!q_al || !kv_al || (q_weight && !aligned16(q_weight)) || (k_weight && !aligned16(k_weight)))
     return fail(UMIC_ERR_ALIGNMENT, "%s: 16-byte alignment of bases / strides", me);
   // rows written: apart from one another
-  const int64_t n_tokens = tokens, width = head_dim;
-  auto apart = [n_tokens, width](int64_t st, int64_t sh, int32_t heads) {
-    return (heads <= 1 || sh >= width) && (n_tokens <= 1 || st >= width);
-  };
-  if ((hq > 0 && !apart(qo_st, qo_sh, hq)) ||
-      (k_pages ? (hk > 1 && pg_sh < head_dim) || pg_ss < head_dim ||
-                     (num_pages > 1 && pg_sp < head_dim)
-               : !apart(ko_st, ko_sh, hk)))
+  if ((hq > 0 && !rows_apart({{tokens, qo_st}, {hq, qo_sh}}, head_dim)) ||
+      !(k_pages ? rows_apart({{num_pages, pg_sp}, {hk, pg_sh}, {page_size, pg_ss}}, head_dim)
+                : rows_apart({{tokens, ko_st}, {hk, ko_sh}}, head_dim)))
     return fail(UMIC_ERR_INVALID_ARG, "%s: output rows overlap", me);
   uint32_t* err = device_error_word();
   if (!err) return fail(UMIC_ERR_DEVICE, "%s: no device error word", me);
