@@ -288,8 +288,10 @@ UMIC_API int umic_qk_norm_mrope_kv(const umic_mrope_args* args, void* stream);
  * past max_pages * page_size is cut there; both set UMIC_DEVERR_BAD_PAGE. What lies
  * behind a request's length in its last page is never used. head_dim 64, 80, 96, 128 or
  * 256, hq a multiple of hkv, page_size a multiple of 16, 16-byte aligned bases and
- * strides; the tiles of 16 tokens that the table's rows allow, times batch and KV heads
- * (groups of more than 8 query heads count once for each 8), below 2^30. The lengths are read on the device: one captured graph serves every length.
+ * strides; the rows of out lie apart (of its two axes, the one of larger stride steps over
+ * all that the other spans); the tiles of 16 tokens that the table's rows allow, times
+ * batch and KV heads (groups of more than 8 query heads count once for each 8), below
+ * 2^30. The lengths are read on the device: one captured graph serves every length.
  * workspace: umic_paged_attention_workspace_bytes() bytes, 16-byte aligned, contents
  * irrelevant before and after; calls that may overlap need one each.
  * Replaces the SDPA call of the decode step (graph.py:76-99), for rows of different

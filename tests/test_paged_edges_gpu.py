@@ -7,7 +7,7 @@ import itertools
 import pytest
 import torch
 
-from umic_b200.kernels import paged_kv_append, qk_norm_mrope_kv
+from umic_b200.kernels import paged_attention, paged_kv_append, qk_norm_mrope_kv
 
 pytestmark = pytest.mark.gpu
 
@@ -67,3 +67,17 @@ def test_single_entries_need_no_stride(cuda):
     paged_kv_append(kp, vp, k, -k, slots)
     assert torch.equal(kp[0, :, 7], k[0]) and torch.equal(vp[0, :, 7], -k[0])
     assert int((pages != 0).sum()) <= 2 * d
+
+
+def test_attention_writes_rows_in_any_order_of_axes(cuda):
+    g = _gen(43)
+    kp, vp = torch.randn(2, 6, 2, 16, 64, generator=g).to(torch.bfloat16).to(cuda)
+    q = torch.randn(3, 8, 64, generator=g).to(torch.bfloat16).to(cuda)
+    table = torch.randperm(6, generator=g).int().view(3, 2).to(cuda)
+    lens = torch.tensor([32, 0, 19], dtype=torch.int32, device=cuda)
+    want = paged_attention(q, kp, vp, table, lens, 0.2)
+    for order, pad in itertools.product(itertools.permutations(range(2)), (0, 8)):
+        out = _ordered((3, 8, 64), order, cuda, pad=pad)
+        out.fill_(9.0)
+        paged_attention(q, kp, vp, table, lens, 0.2, out=out)
+        assert torch.equal(out, want)

@@ -35,3 +35,16 @@ def _input(qo=(512, 128), ko=(256, 128), pages=None, num=8, page=16, d=128):
 def test_input_rows_that_meet_are_refused(kw):
     assert _input(**kw) == 1
     assert "overlap" in _lib.last_message()
+
+
+def _attend(out, batch=3, hq=4):
+    args = _lib.pack_paged_attention_args(
+        F, F, F, 0, 0, F, F, F, 0, F, 512, 128, 4096, 2048, 128, 8, 16, 4, 4, *out, batch, 1 << 30,
+        hq, 2, 128, 0, 0.1)
+    return _lib.lib().umic_paged_attention(args, None)
+
+
+@pytest.mark.parametrize("out", [(128, 128), (384, 128), (128, 256), (504, 128), (136, 128)])
+def test_attention_rows_that_meet_are_refused(out):
+    assert _attend(out) == 1
+    assert "overlap" in _lib.last_message()

@@ -1125,7 +1125,7 @@ extern "C" int umic_paged_attention(const umic_paged_attention_args* args, void*
   if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out) ||
       q_sb % 8 || q_sh % 8 || o_sb % 8 || o_sh % 8 || pg_sp % pe || pg_sh % pe || pg_ss % pe)
     return fail(UMIC_ERR_ALIGNMENT, "%s: 16-byte alignment of bases / strides", me);
-  if ((hq > 1 && o_sh < head_dim) || (batch > 1 && o_sb < head_dim))
+  if (!rows_apart({{batch, o_sb}, {hq, o_sh}}, head_dim))
     return fail(UMIC_ERR_INVALID_ARG, "%s: output rows overlap", me);
   const size_t need = umic_paged_attention_workspace_bytes(batch, hq, hkv, head_dim, max_pages,
                                                            page_size, cache_dtype);
