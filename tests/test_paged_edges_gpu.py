@@ -81,3 +81,35 @@ def test_attention_writes_rows_in_any_order_of_axes(cuda):
         out.fill_(9.0)
         paged_attention(q, kp, vp, table, lens, 0.2, out=out)
         assert torch.equal(out, want)
+
+
+# ------------------------------------------------------------ longest rows
+
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_attention_over_the_longest_row(cuda, e4m3):
+    """A row of 2^31 - 16 tokens (262657 entries that name one page of 8176), beside a short
+    one. All scores are 0 and V of a dim is the same in every token, so the output is that
+    value and the lse the length's logarithm.
+
+    Bounds: a warp sums its share of the line, one product of 16 tokens after the other, each
+    off by at most a step of the running sum (2^-23), and the output is rounded once (2^-8).
+    The weights are 1 and their sums whole numbers, exact in a lane; about 200 partial sums
+    are joined (2^-24 of the sum each), and the logarithm, 22 at most, is good to four half
+    steps.
+    """
+    page, width, d = 8176, 262657, 64
+    n = page * width
+    assert n == 2 ** 31 - 16
+    dt = torch.float8_e4m3fn if e4m3 else torch.bfloat16
+    dims = (torch.arange(d) % 3).float()
+    kp = torch.ones(1, 1, page, d).to(dt).to(cuda)
+    vp = dims.expand(1, 1, page, d).contiguous().to(dt).to(cuda)
+    table = torch.zeros(2, width, dtype=torch.int32, device=cuda)
+    lens = torch.tensor([n, 40], dtype=torch.int32, device=cuda)
+    q = torch.zeros(2, 3, d, dtype=torch.bfloat16, device=cuda)
+    out, lse = paged_attention(q, kp, vp, table, lens, 0.3, return_lse=True)
+    warps = torch.cuda.get_device_properties(cuda).multi_processor_count * 8
+    rel = 2.0 ** -8 + (n / 16 / warps + 200) * 2.0 ** -23
+    assert bool(((out.cpu().float() - dims).abs() <= dims * rel).all())
+    want = lens.cpu().double().log()[:, None].expand(2, 3)
+    assert bool(((lse.cpu().double() - want).abs() <= (200 + 4 * 22) * 2.0 ** -24).all())

@@ -323,7 +323,10 @@ __global__ void __launch_bounds__(Shape<D, kE4m3, NT>::kWarps * 32, 1)
   using R = Rows<D, kE4m3, NT>;
   constexpr int kWarps = S::kWarps, kStages = S::kStages, kBlocks = S::kBlocks;
   constexpr int kThreads = kWarps * 32, MT = S::MT, kTile = S::kTile;
-  auto tiles_of = [](int len) { return (len + kTile - 1) / kTile; };
+  // unsigned: rows may reach up to 2^31 - 16 tokens
+  auto tiles_of = [](int len) {
+    return static_cast<int>((static_cast<uint32_t>(len) + kTile - 1) / kTile);
+  };
   extern __shared__ char smem[];
   char* const ring_mem = smem + (-smem_addr(smem) & 511u);  // rows lie on their own size
   // request (-1: no more tiles), segment, valid rows (a byte per subtile) and flags, tiles
