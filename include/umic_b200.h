@@ -246,8 +246,8 @@ UMIC_API int umic_paged_plan(const int32_t* kv_lens, const int32_t* new_tokens,
  * may be q itself, with its strides, but not lie across it otherwise) gets the rotated q.
  * With k_pages, K and V of token t are written at slots[t] (-1: not written; other slots
  * outside the pool set UMIC_DEVERR_BAD_PAGE and are not written; two tokens must not
- * share a slot), rounded once to cache_dtype (e4m3 saturates at +-448; scales are normal
- * positive numbers); without, the rotated k goes to k_out (which may be k) and v is not
+ * share a slot), rounded once to cache_dtype (e4m3: the fp32 value over its head's scale,
+ * a normal positive number, saturated at +-448); without, the rotated k goes to k_out (which may be k) and v is not
  * touched. Bases are 16-byte aligned, strides multiples of 16 bytes. Rows that are written
  * lie apart: the axes of q_out, k_out and the pages may come in any order, but each steps
  * over all that those of smaller stride span (UMIC_ERR_INVALID_ARG otherwise).

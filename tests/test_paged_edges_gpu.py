@@ -113,3 +113,49 @@ def test_attention_over_the_longest_row(cuda, e4m3):
     assert bool(((out.cpu().float() - dims).abs() <= dims * rel).all())
     want = lens.cpu().double().log()[:, None].expand(2, 3)
     assert bool(((lse.cpu().double() - want).abs() <= (200 + 4 * 22) * 2.0 ** -24).all())
+
+
+# ------------------------------------------------------- borders of e4m3
+
+def _border_scales():
+    """(scales, values) fp32 of quotients value / scale that lie on or next to the middle of
+    two e4m3 values: value 128 .. 255 over 17, 19 .. 31, and the neighbours of that scale."""
+    x = torch.arange(128, 256).float().repeat_interleave(8)
+    s = x / torch.arange(17, 33, 2).float().repeat(128)
+    up, down = (torch.nextafter(s, s + d) for d in (1.0, -1.0))
+    return torch.cat((down, s, up)), x.repeat(3)
+
+
+def _stored(x, s):
+    """The page's bytes for x over s: the quotient in fp32, saturated, rounded to e4m3."""
+    return (x / s).clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8)
+
+
+@pytest.mark.parametrize("form", ["append", "rotated", "normed"])
+def test_e4m3_pages_hold_the_rounded_quotient(cuda, form):
+    """K and V in e4m3 pages are the value divided by its head's scale, not multiplied by the
+    scale's rounded inverse, bit for bit: as they are, rotated by position 0, and (V) beside a
+    normed K. A product with the inverse stores the neighbour of some of these quotients."""
+    scale, x = _border_scales()
+    assert bool((_stored(x, scale) != _stored(x * (1 / scale), torch.ones_like(x))).any())
+    hk, d = len(x), 16
+    rows = x[:, None] * 2.0 ** -torch.arange(d).float()  # the border at every exponent, then
+    rows[:, 1::2] *= -1                                  # smaller values, subnormal at last
+    k = rows.to(torch.bfloat16)[None].repeat(3, 1, 1)
+    k[1] *= 8  # up to 248 and, over the border of the type, saturated
+    k[2] *= 32
+    pages = torch.zeros(2, 1, hk, 16, d, dtype=torch.uint8, device=cuda).view(torch.float8_e4m3fn)
+    slots = torch.tensor([3, 0, 9], dtype=torch.int32, device=cuda)
+    kd, s = k.to(cuda), scale.to(cuda)
+    if form == "append":
+        paged_kv_append(pages[0], pages[1], kd, -kd, slots, k_scale=s, v_scale=s)
+    else:
+        w = torch.ones(d, dtype=torch.bfloat16, device=cuda) if form == "normed" else None
+        qk_norm_mrope_kv(None, kd, -kd, torch.zeros(1, 3, dtype=torch.int32, device=cuda),
+                         torch.ones(8, device=cuda), (8,), k_weight=w, k_pages=pages[0],
+                         v_pages=pages[1], slots=slots, k_scale=s, v_scale=s)
+    want = _stored(k.float(), scale[:, None])
+    got = pages.view(torch.uint8)[:, 0][:, :, [3, 0, 9]].transpose(1, 2).cpu()
+    assert torch.equal(got[1], want ^ 0x80)
+    if form != "normed":
+        assert torch.equal(got[0], want)

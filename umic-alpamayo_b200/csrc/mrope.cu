@@ -20,11 +20,11 @@
 // out among the row groups' lanes and handed round by shuffles, times the norm's weights,
 // when the warp comes to the q rows and to the k rows:
 //   out[i] = rstd (x[i] w[i] cos - x[i + r/2] w[i + r/2] sin), and so on.
-// Measured: 24800 tokens of 32 + 8 + 8 heads x 128 into e4m3 pages 101 us (0.85 of measured
-// HBM, issue slots 0.68 busy), 3100 into bf16 pages 14.5 us (0.80), 16384 x (16 + 16) x 80
+// Measured: 24800 tokens of 32 + 8 + 8 heads x 128 into e4m3 pages 103 us (0.83 of measured
+// HBM), 3100 into bf16 pages 14.5 us (0.80), 16384 x (16 + 16) x 80
 // without norm or cache 37.5 us (0.68), 6200 tokens appended as they are 9.7 us (0.80), 8
 // tokens 3.2 us. (Whole tokens or shares of one to a warp instead of equal runs: 108 and
-// 17.7 us for the first two.)
+// 17.7 us for the first two, before the quotients below were exact and it took 101.)
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -85,6 +85,28 @@ __device__ __forceinline__ uint2 pack8_e4m3(const float (&f)[8]) {
                     make_float2(f[2 * i], f[2 * i + 1]), __NV_SATFINITE, __NV_E4M3))
                 << (i % 2 * 16);
   return make_uint2(w[0], w[1]);
+}
+
+// A lane's values over the scale of their head, for e4m3. The product with the scale's
+// rounded inverse alone carries some quotients over the border between two e4m3 values; its
+// remainder, times the inverse again (Markstein's correction, 1990), puts it right for less
+// than a division: 24800 tokens of 32 + 8 + 8 heads take 101 us with the product, 103 us so
+// and 118 us with divisions, 24800 appended as they are 27, 33 and 45 us. Before its last
+// rounding the quotient is off by 2^-46 of itself; the quotients of bf16 values (above
+// 2^-100, where the remainder is normal) come no nearer to the middle between a border and
+// the float beside it, so they are stored as after a division, bit for bit.
+__device__ __forceinline__ void divide(float (&x)[8], float (&y)[8], float scale) {
+  const float inv = 1.f / scale;
+  auto over = [scale, inv](float v) {
+    // 512 saturates all the same, and the remainder of an infinity would be NaN
+    const float q = fminf(fmaxf(v * inv, -512.f), 512.f);
+    return fmaf(fmaf(-q, scale, v), inv, q);
+  };
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    x[i] = over(x[i]);
+    y[i] = over(y[i]);
+  }
 }
 
 // The sum over a row's lanes.
@@ -281,7 +303,6 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kWork)) mrope_kernel(M
           ss = row_sum<TPH>(ss, mine);
           f = rsqrtf(ss * inv_d + eps);
         }
-        if (e4m3 && a.k_scale && row < a.hk) f /= __ldg(a.k_scale + row);
         if (turns) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
@@ -296,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kWork)) mrope_kernel(M
             y[i] *= yc[i];
           }
         }
-        if (wt || e4m3) {
+        if (wt) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             x[i] *= f;
@@ -305,6 +326,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kWork)) mrope_kernel(M
         }
         if (row < heads) {
           if (e4m3) {
+            if (a.k_scale) divide(x, y, __ldg(a.k_scale + row));
             *reinterpret_cast<uint2*>(dst + lo) = pack8_e4m3(x);
             *reinterpret_cast<uint2*>(dst + hi) = pack8_e4m3(y);
           } else {
@@ -331,12 +353,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kWork)) mrope_kernel(M
           float x[8], y[8];
           unpack8(xv, x);
           unpack8(yv, y);
-          const float f = a.v_scale ? 1.f / __ldg(a.v_scale + row) : 1.f;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            x[i] *= f;
-            y[i] *= f;
-          }
+          if (a.v_scale) divide(x, y, __ldg(a.v_scale + row));
           *reinterpret_cast<uint2*>(dst + lo) = pack8_e4m3(x);
           *reinterpret_cast<uint2*>(dst + hi) = pack8_e4m3(y);
         } else {
