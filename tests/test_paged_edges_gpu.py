@@ -7,6 +7,7 @@ import itertools
 import pytest
 import torch
 
+from oracle import paged as oracle
 from umic_b200.kernels import paged_attention, paged_kv_append, qk_norm_mrope_kv
 
 pytestmark = pytest.mark.gpu
@@ -159,3 +160,103 @@ def test_e4m3_pages_hold_the_rounded_quotient(cuda, form):
     assert torch.equal(got[1], want ^ 0x80)
     if form != "normed":
         assert torch.equal(got[0], want)
+
+
+# ------------------------------------------------------------- long walks
+
+WALKS = [
+    # hq, hk, d, rotary sections, interleaved
+    (32, 8, 128, (24, 20, 20), True),
+    (16, 16, 80, (20, 20), False),
+    (12, 3, 96, (8, 4, 4), True),
+    (6, 2, 256, (128,), False),
+]
+
+
+@pytest.mark.parametrize("walk", WALKS, ids=lambda w: "x".join(map(str, w[:3])))
+@pytest.mark.parametrize("tokens", [9001, 24800])
+@pytest.mark.parametrize("form", ["bf16", "e4m3", "plain", "append", "append_e4m3"])
+def test_input_of_many_tokens_a_warp(cuda, walk, tokens, form):
+    """So many tokens that a warp walks over several (10 and more of 24800): every row and
+    every slot has the bits of calls on 400 tokens, of which a warp sees no more than two, and
+    tokens picked at random agree with the 64-bit oracle. Values differ by token, head, dim and
+    kind of row; slots are shuffled, some tokens have none, and other slots keep what they held.
+    """
+    hq, hk, d, sections, inter = walk
+    e4m3, append = "e4m3" in form, "append" in form
+    g = torch.Generator(device=cuda).manual_seed(tokens + d)
+    qkv = torch.randn(tokens, hq + 2 * hk, d, generator=g, device=cuda).to(torch.bfloat16)
+    q, k, v = qkv.split((hq, hk, hk), 1)
+    half = sum(sections)
+    inv = (1e6 ** (-torch.arange(half, device=cuda) / half)).float()
+    pos = torch.randint(0, 32768, (len(sections), tokens), generator=g, device=cuda)
+    weights = (1 + 0.2 * torch.randn(2, d, generator=g, device=cuda)).to(torch.bfloat16)
+    norm = dict(q_weight=weights[0], k_weight=weights[1]) if form != "plain" else {}
+    page = 16
+    pages = tokens // page + 3
+    slots = torch.randperm(pages * page, generator=g, device=cuda)[:tokens].int()
+    slots[3::11] = -1
+    scales = (0.5 + torch.rand(2, hk, generator=g, device=cuda)) / 40
+
+    def filled():
+        x = torch.full((2, pages, hk, page, d), 0x3c, dtype=torch.uint8, device=cuda)
+        return x.view(torch.float8_e4m3fn) if e4m3 else x.to(torch.bfloat16)
+
+    def call(pool, a, b):
+        kwargs = {}
+        if e4m3:
+            kwargs = dict(k_scale=scales[0], v_scale=scales[1])
+        if append:
+            return paged_kv_append(pool[0], pool[1], k[a:b], v[a:b], slots[a:b], **kwargs)
+        if form != "plain":
+            kwargs.update(k_pages=pool[0], v_pages=pool[1], slots=slots[a:b])
+        return qk_norm_mrope_kv(q[a:b], k[a:b], v[a:b], pos[:, a:b], inv, sections,
+                                interleaved=inter, **norm, **kwargs)
+
+    pool, parts = filled(), filled()
+    whole = call(pool, 0, tokens)
+    pieces = [call(parts, a, min(a + 400, tokens)) for a in range(0, tokens, 400)]
+    as_bytes = lambda x: x.view(torch.uint8) if e4m3 else x  # noqa: E731
+    assert torch.equal(as_bytes(pool), as_bytes(parts))
+    free = torch.ones(pages * page, dtype=torch.bool, device=cuda)
+    free[slots[slots >= 0].long()] = False
+    untouched = as_bytes(pool).transpose(2, 3).flatten(1, 2)[:, free]
+    assert bool((untouched == 0x3c).all())
+    on = torch.nonzero(slots >= 0)[:, 0]
+    at = slots[on].long()
+    if not e4m3:
+        stored = pool[1].transpose(1, 2).flatten(0, 1)
+        if form != "plain":
+            assert torch.equal(stored[at], v[on])
+        if append:
+            assert torch.equal(pool[0].transpose(1, 2).flatten(0, 1)[at], k[on])
+    elif append:
+        for kind, x in enumerate((k, v)):
+            want = (x[on].float() / scales[kind][:, None]).clamp(-448, 448)
+            got = as_bytes(pool)[kind].transpose(1, 2).flatten(0, 1)[at]
+            assert torch.equal(got, want.to(torch.float8_e4m3fn).view(torch.uint8))
+    if append:
+        return
+    assert torch.equal(whole[0], torch.cat([x[0] for x in pieces]))
+    pick = torch.randperm(tokens, generator=_gen(d))[:300].to(cuda)
+    args = (pos[:, pick], inv, sections, inter)
+    u = 2.0 ** -24  # 40 roundings in fp32 of |a| + |b|, then half a step of the output's type
+    y, mag = oracle.norm_mrope(q[pick], norm.get("q_weight"), 1e-6, *args)
+    bound = mag * 40 * u
+    bound = bound + (y.abs() + bound) * 2.0 ** -8
+    assert bool(((whole[0][pick].cpu().double() - y).abs() <= bound).all())
+    y, mag = oracle.norm_mrope(k[pick], norm.get("k_weight"), 1e-6, *args)
+    if form == "plain":
+        assert torch.equal(whole[1], torch.cat([x[1] for x in pieces]))
+        got, scale = whole[1][pick].cpu().double(), 1.0
+    else:
+        there = (slots[pick] >= 0).cpu()
+        y, mag = y[there], mag[there]
+        got = as_bytes(pool)[0].transpose(1, 2).flatten(0, 1)[slots[pick].long()[there.to(cuda)]]
+        got = (got.view(torch.float8_e4m3fn).float() if e4m3 else got).cpu().double()
+        scale = scales[0].cpu().double()[:, None] if e4m3 else 1.0
+    bound = mag * 40 * u / scale
+    y = (y / scale).clamp(-448, 448) if e4m3 else y
+    half_step = torch.clamp((y.abs() + bound) * 2.0 ** -4, min=2.0 ** -10) if e4m3 else \
+        (y.abs() + bound) * 2.0 ** -8
+    assert bool(((got - y).abs() <= bound + half_step).all())
