@@ -8,6 +8,7 @@ import pytest
 import torch
 
 from oracle import paged as oracle
+from umic_b200 import _lib
 from umic_b200.kernels import paged_attention, paged_kv_append, qk_norm_mrope_kv
 
 pytestmark = pytest.mark.gpu
@@ -260,3 +261,22 @@ def test_input_of_many_tokens_a_warp(cuda, walk, tokens, form):
     half_step = torch.clamp((y.abs() + bound) * 2.0 ** -4, min=2.0 ** -10) if e4m3 else \
         (y.abs() + bound) * 2.0 ** -8
     assert bool(((got - y).abs() <= bound + half_step).all())
+
+
+# ----------------------------------------------------------------- streams
+
+@pytest.mark.parametrize("raw", [True, False])
+def test_calls_go_to_the_current_stream(cuda, raw, monkeypatch):
+    """The handle passed to the library is torch's current stream: the default one, a side
+    stream, the one that a graph is captured on; with and without torch's short cut to it."""
+    if not raw:
+        monkeypatch.setattr(_lib, "_raw_stream", None)
+    anywhere = torch.device("cuda")
+    side = torch.cuda.Stream()
+    for dev in (cuda, anywhere):
+        assert _lib.stream_ptr(dev) == torch.cuda.current_stream(cuda).cuda_stream
+        with torch.cuda.stream(side):
+            assert _lib.stream_ptr(dev) == side.cuda_stream
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        assert _lib.stream_ptr(cuda) == torch.cuda.current_stream(cuda).cuda_stream != 0
+        torch.zeros(1, device=cuda)

@@ -159,17 +159,16 @@ def last_message() -> str:
     return m.decode() if m else ""
 
 
-def stream_ptr(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
-
-
-# The current stream's handle without a Stream object around it (1.5 us less per call),
+# The current stream's handle without a Stream object around it (0.1 us a call for 2.2),
 # where this torch has it.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-if _raw_stream is not None:
-    def stream_ptr(device: torch.device) -> int:  # noqa: F811
-        index = device.index
-        return _raw_stream(torch.cuda.current_device() if index is None else index)
+
+
+def stream_ptr(device: torch.device) -> int:
+    if _raw_stream is None:
+        return torch.cuda.current_stream(device).cuda_stream
+    index = device.index
+    return _raw_stream(torch.cuda.current_device() if index is None else index)
 
 
 def call(name: str, device: torch.device, *args) -> None:
