@@ -23,6 +23,15 @@ Used to capture a single kernel under ncu. Modes and shapes:
                  (mask packing + umic_attention_rows)
   attn_nomask    the same without a mask
   attn_sdpa      the same shape and mask through torch SDPA (what transformers runs)
+  paged_plan     step plan of rows=1024 requests of up to 4100 tokens on pages of 32, one
+                 token each, a tenth of them ending
+  paged_prompts  the same of rows=32 requests, 80 % new, with prompts of 1550 to 3100 tokens
+  paged_input    attention input of rows=3100 tokens x (32 + 8 + 8) x 128: norm, three axes,
+                 bf16 pages;  paged_input_e4m3: rows=24800 tokens into e4m3 pages
+  paged_vision   two axes, no norm, no cache: rows=16384 patches x (16 + 16) x 80
+  paged_append   rows=6200 finished tokens x 8 x 128 into bf16 pages
+  paged_attn     paged attention of rows=8 requests of 3164 tokens, 32 / 8 heads x 128
+  paged_attn_e4m3  of rows=256 requests of 1 to 4096 tokens, 16 / 8 heads x 128, e4m3 pages
 Inputs are seeded random tensors created on cuda:0 before the launches. Without --time
 the first call runs alone and the next --iters calls run inside the NVTX range "drv"
 (`ncu --nvtx --nvtx-include "drv/"` captures just those). --time runs
@@ -188,7 +197,70 @@ def make(mode: str, rows: int | None):
                               CFG5_EXPERT["num_key_value_heads"], PREFILL_TOKENS,
                               CFG5_EXPERT["head_dim"], dev)
         return lambda: flow_sample(expert, cache, PREFILL_TOKENS, x0, graph=True)
+    if mode.startswith("paged_"):
+        return _make_paged(mode, rows, dev, bf)
     raise SystemExit(f"unknown mode {mode}")
+
+
+def _make_paged(mode: str, rows: int | None, dev, bf):
+    from umic_b200.kernels import paged_attention, paged_kv_append, paged_plan, qk_norm_mrope_kv
+
+    e4m3 = mode.endswith("e4m3")
+
+    def pool(pages, page, heads):
+        x = torch.randn(2, pages, heads, page, 128, device=dev, dtype=bf)
+        if not e4m3:
+            return x[0], x[1], {}
+        x = (x * 48).clamp_(-448, 448).to(torch.float8_e4m3fn)
+        one = torch.full((heads,), 1 / 48, device=dev)
+        return x[0], x[1], {"k_scale": one, "v_scale": one}
+
+    if mode in ("paged_plan", "paged_prompts"):
+        r, page, width = (rows or 1024, 32, 129) if mode == "paged_plan" else (rows or 32, 64, 52)
+        if mode == "paged_plan":
+            lens = torch.randint(1, 4100, (r,), device=dev)
+            new = torch.where(torch.rand(r, device=dev) < 0.1, -lens, 1)
+            capacity = r
+        else:
+            lens = torch.randint(1, 200, (r,), device=dev) * (torch.rand(r, device=dev) < 0.2)
+            new = torch.randint(1550, 3101, (r,), device=dev)
+            capacity = 3100 * r
+        order = torch.randperm(r * width, device=dev).int()
+        table, ring = order.view(r, width).clone(), order.flip(0).contiguous()
+        span = torch.tensor([0, r * width], device=dev)
+        lens, new = lens.int(), new.int()
+        return lambda: paged_plan(lens, new, table, ring, span, page, capacity)
+    if mode in ("paged_attn", "paged_attn_e4m3"):
+        b, longest, hq, hk = (rows or 256, 4096, 16, 8) if e4m3 else (rows or 8, 3164, 32, 8)
+        lens = torch.randint(1, longest + 1, (b,), device=dev) if e4m3 else \
+            torch.full((b,), longest, device=dev)
+        width = -(-longest // 64)
+        kp, vp, scales = pool(b * width, 64, hk)
+        table = torch.randperm(b * width, device=dev).int().view(b, width)
+        q = torch.randn(b, hq, 128, device=dev, dtype=bf)
+        lens = lens.int()
+        return lambda: paged_attention(q, kp, vp, table, lens, 128 ** -0.5, **scales)
+    if mode == "paged_vision":
+        t = rows or 16384
+        qkv = torch.randn(t, 48, 80, device=dev, dtype=bf)
+        at = torch.arange(t, device=dev) % 1024
+        pos = torch.stack((at // 32, at % 32))
+        inv = (1e4 ** (-(torch.arange(40, device=dev) % 20) / 20)).float()
+        return lambda: qk_norm_mrope_kv(qkv[:, :16], qkv[:, 16:32], None, pos, inv, (20, 20))
+    if mode not in ("paged_input", "paged_input_e4m3", "paged_append"):
+        raise SystemExit(f"unknown mode {mode}")
+    t = rows or {"paged_input": 3100, "paged_input_e4m3": 24800, "paged_append": 6200}[mode]
+    qkv = torch.randn(t, 48, 128, device=dev, dtype=bf)
+    kp, vp, scales = pool(-(-t // 32), 32, 8)
+    slots = torch.randperm(-(-t // 32) * 32, device=dev)[:t].int()
+    if mode == "paged_append":
+        return lambda: paged_kv_append(kp, vp, qkv[:, 32:40], qkv[:, 40:], slots, **scales)
+    w = torch.ones(128, device=dev, dtype=bf)
+    pos = torch.randint(0, 32768, (3, t), device=dev)
+    inv = (1e6 ** (-torch.arange(64, device=dev) / 64)).float()
+    return lambda: qk_norm_mrope_kv(
+        qkv[:, :32], qkv[:, 32:40], qkv[:, 40:], pos, inv, (24, 20, 20), interleaved=True,
+        q_weight=w, k_weight=w, k_pages=kp, v_pages=vp, slots=slots, **scales)
 
 
 def main() -> None:

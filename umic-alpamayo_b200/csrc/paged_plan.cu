@@ -20,7 +20,11 @@ namespace {
 constexpr int kMostThreads = 1024;
 constexpr int64_t kMaxRequests = 8192;
 constexpr int kMostEach = kMaxRequests / kMostThreads;  // requests a thread scans, at most
-constexpr int kFew = 4;  // pages of a request that the scanning thread moves itself
+// Pages of a request that the scanning thread moves itself. Requests that take two or three
+// gain by it (64, 512 and 1024 prompts of 32 tokens on pages of 16: 6.6, 9.4 and 10.5 us,
+// against 6.9, 10.3 and 11.2 with one), steps of one token lose 0.2 us; with 16 all lose 1 to
+// 1.5 us.
+constexpr int kFew = 4;
 
 struct PlanArgs {
   const int32_t* lens;
@@ -318,10 +322,14 @@ extern "C" int umic_paged_plan(const int32_t* kv_lens, const int32_t* new_tokens
     cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                          static_cast<int>(kMaxRequests * (sizeof(int4) + sizeof(int32_t))));
   });
-  // One small CTA while four tokens a thread and a request a thread cover the step; else
-  // large ones, more while there are 4096 tokens or 128 requests for each
-  // (1024 requests of one token, a tenth of them ending: 11 us against 17 in one CTA).
-  const int threads = requests <= 128 && capacity <= 512 ? 128 : kMostThreads;
+  // One small CTA while four tokens a thread and a request a thread cover the step and its
+  // four warps hide their look-ups: against 1024 threads, 8 requests of one token take 5.4 us
+  // to 6.0, 32 take 6.45 to 6.65, 48 take 6.9 to 6.85, 128 take 9.1 to 7.6, and one prompt of
+  // 512 tokens 3.8 to 4.5. Else large ones, twice as many while there are more than 4096
+  // tokens or 128 requests for each: 1, 2, 4 and 8 CTAs take 12.5, 11.3, 10.5 and 10.2 us for
+  // 1024 requests, 15.4 to 10.3 with a tenth of them ending, 8.5, 7.0, 5.7 and 5.8 for four
+  // prompts of 3100 tokens, 42, 24, 14 and 10 for 32.
+  const int threads = requests <= 40 && capacity <= 512 ? 128 : kMostThreads;
   int ctas = 1;
   while (threads == kMostThreads && ctas < 8 && (capacity > 4096 * ctas || requests > 128 * ctas))
     ctas *= 2;
