@@ -247,15 +247,16 @@ UMIC_API int umic_paged_plan(const int32_t* kv_lens, const int32_t* new_tokens,
  * With k_pages, K and V of token t are written at slots[t] (-1: not written; other slots
  * outside the pool set UMIC_DEVERR_BAD_PAGE and are not written; two tokens must not
  * share a slot), rounded once to cache_dtype (e4m3: the fp32 value over its head's scale,
- * a normal positive number, saturated at +-448); without, the rotated k goes to k_out (which may be k) and v is not
- * touched. Bases are 16-byte aligned, strides multiples of 16 bytes. Rows that are written
+ * a normal positive number, saturated at +-448); without, the rotated k goes to k_out
+ * (which may be k) and v is not touched. Bases are 16-byte aligned, strides multiples of 16 bytes. Rows that are written
  * lie apart: the axes of q_out, k_out and the pages may come in any order, but each steps
  * over all that those of smaller stride span (UMIC_ERR_INVALID_ARG otherwise).
  * The angle of pair i, which holds elements i and i + rotary_dim / 2, is
  * positions[axis(i), t] * inv_freq[i], computed in 64 bits: axis(i) = the section of
  * (s0, s1, s2) that i falls in, or with interleaved != 0 (t h w t h w ... t t) axis
- * i % axes while i < axes * s_axis, else axis 0. Sections sum to rotary_dim / 2; cos
- * and sin are multiplied by scaling; elements from rotary_dim on are passed through.
+ * i % axes while i < axes * s_axis, else axis 0 (so an axis behind the first turns at
+ * most every axes-th pair, however large its section). Sections sum to rotary_dim / 2;
+ * cos and sin are multiplied by scaling; elements from rotary_dim on are passed through.
  * positions [axes, tokens] through (p_sa, p_st; 0 broadcasts), int32 or int64
  * (pos_bytes 4 or 8). rotary_dim 0: no rotation (positions, inv_freq unused). hq 0:
  * no q. head_dim a multiple of 16 up to 256, rotary_dim a multiple of 16 up to it.
@@ -284,14 +285,18 @@ UMIC_API int umic_qk_norm_mrope_kv(const umic_mrope_args* args, void* stream);
  * out[b, h] = softmax(scale * q[b, h] . k_j over j < kv_lens[b]) . v_j. q and out
  * [batch, hq, head_dim] through (sb, sh); lse [batch, hq] fp32 (natural log of the sum
  * of exponentials; NULL = not wanted). A request without tokens comes out as zeros,
- * lse -inf. A table entry outside the pool is left out of its request's sums, a length
- * past max_pages * page_size is cut there; both set UMIC_DEVERR_BAD_PAGE. What lies
- * behind a request's length in its last page is never used. head_dim 64, 80, 96, 128 or
- * 256, hq a multiple of hkv, page_size a multiple of 16, 16-byte aligned bases and
- * strides; the rows of out lie apart (of its two axes, the one of larger stride steps over
- * all that the other spans); the tiles of 16 tokens that the table's rows allow, times
- * batch and KV heads (groups of more than 8 query heads count once for each 8), below
- * 2^30. The lengths are read on the device: one captured graph serves every length.
+ * lse -inf. All sums are fp32. Over bf16 pages each weight is held to 2^-17 of itself;
+ * over e4m3 pages to 2^-11 (one fp16 value; the sum of weights and the lse take it in
+ * fp32), and elements of q below 2^-14 of their row's largest to 2^-25 of that. A NaN of a
+ * token in use reaches its rows as NaN, an infinity in V as an infinity or NaN. A table
+ * entry outside the pool is left out of its request's sums, a length past max_pages *
+ * page_size is cut there; both set UMIC_DEVERR_BAD_PAGE. What lies behind a request's
+ * length in its last page is never used. head_dim 64, 80, 96, 128 or 256, hq a multiple of
+ * hkv, page_size a multiple of 16, 16-byte aligned bases and strides; the rows of out lie
+ * apart (of its two axes, the one of larger stride steps over all that the other spans);
+ * the tiles of 16 tokens that the table's rows allow, times batch and KV heads (groups of
+ * more than 8 query heads count once for each 8), below 2^30. The lengths are read on the
+ * device: one captured graph serves every length.
  * workspace: umic_paged_attention_workspace_bytes() bytes, 16-byte aligned, contents
  * irrelevant before and after; calls that may overlap need one each.
  * Replaces the SDPA call of the decode step (graph.py:76-99), for rows of different

@@ -280,3 +280,39 @@ def test_calls_go_to_the_current_stream(cuda, raw, monkeypatch):
     with torch.cuda.graph(torch.cuda.CUDAGraph()):
         assert _lib.stream_ptr(cuda) == torch.cuda.current_stream(cuda).cuda_stream != 0
         torch.zeros(1, device=cuda)
+
+
+# ---------------------------------------------------------------- sections
+
+@pytest.mark.parametrize("sections", [(24, 20, 20), (10, 27, 27), (0, 32, 32), (64, 0, 0)])
+def test_interleaved_sections_past_the_frequencies(cuda, sections):
+    """Interleaved sections of every reach turn what the documented rule says."""
+    g = _gen(51)
+    x = torch.randn(64, 3, 128, generator=g).to(torch.bfloat16)
+    pos = torch.randint(0, 32768, (3, 64), generator=g)
+    inv = 1e6 ** (-torch.arange(64) / 64)
+    got, _ = qk_norm_mrope_kv(x.to(cuda), x[:, :1].to(cuda), None, pos.to(cuda), inv.to(cuda),
+                              sections, interleaved=True)
+    y, mag = oracle.norm_mrope(x, None, 0.0, pos, inv, sections, True)
+    bound = mag * 40 * 2.0 ** -24  # roundings in fp32, then half a step of bf16
+    bound = bound + (y.abs() + bound) * 2.0 ** -8
+    assert bool(((got.cpu().double() - y).abs() <= bound).all())
+
+
+# --------------------------------------------------------------- infinity
+
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_infinite_values_reach_their_rows(cuda, sign):
+    """An infinity in V of a token in use comes out as an infinity or NaN in its dim of the
+    heads of its KV head, and nowhere else."""
+    g = _gen(53)
+    kp, vp = torch.randn(2, 4, 2, 16, 64, generator=g).to(torch.bfloat16).to(cuda)
+    q = torch.randn(2, 6, 64, generator=g).to(torch.bfloat16).to(cuda)
+    table = torch.arange(4, dtype=torch.int32, device=cuda).view(2, 2)
+    lens = torch.tensor([32, 20], dtype=torch.int32, device=cuda)
+    clean = paged_attention(q, kp, vp, table, lens, 0.1)
+    vp[1, 1, 3, 17] = sign * float("inf")
+    out = paged_attention(q, kp, vp, table, lens, 0.1)
+    assert not bool(out[0, 3:, 17].isfinite().any())
+    out[0, 3:, 17] = clean[0, 3:, 17]
+    assert torch.equal(out, clean)

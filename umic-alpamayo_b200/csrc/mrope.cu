@@ -16,15 +16,17 @@
 // so the rotation needs no exchange and the norm log2(TPH) shuffles. The row groups (32 / TPH
 // rows of one kind: q, k or v) of all tokens form one line, and every resident warp walks
 // over an equal run of it; each lane copies its own pieces of the next kDepth groups, across
-// tokens, into shared memory with asynchronous loads. A token's angles are made once per warp, shared
-// out among the row groups' lanes and handed round by shuffles, times the norm's weights,
-// when the warp comes to the q rows and to the k rows:
+// tokens, into shared memory with asynchronous loads. A token's angles are made once per warp,
+// shared out among the row groups' lanes and handed round by shuffles, times the norm's
+// weights, when the warp comes to the q rows and to the k rows:
 //   out[i] = rstd (x[i] w[i] cos - x[i + r/2] w[i + r/2] sin), and so on.
 // Measured: 24800 tokens of 32 + 8 + 8 heads x 128 into e4m3 pages 103 us (0.83 of measured
-// HBM), 3100 into bf16 pages 14.5 us (0.80), 16384 x (16 + 16) x 80
-// without norm or cache 37.5 us (0.68), 6200 tokens appended as they are 9.7 us (0.80), 8
-// tokens 3.2 us. (Whole tokens or shares of one to a warp instead of equal runs: 108 and
-// 17.7 us for the first two, before the quotients below were exact and it took 101.)
+// HBM), 3100 into bf16 pages 14.5 us (0.80), 6200 tokens appended as they are 9.7 us (0.80),
+// into e4m3 pages 11.5 us (0.50), 24800 of them 33 us (0.71), 8 tokens 3.2 us. 16384 x (16 +
+// 16) x 80 without norm or cache 37.5 us (0.68): latency, at the 16 warps an SM that 128
+// registers allow (issue slots 0.62 busy, DRAM 0.40; the angles' products are made for q and
+// again for k, and a sixth of the lanes holds no row). (Whole tokens or shares of one to a warp
+// instead of equal runs: 108 and 17.7 us for the first two, while the first took 101.)
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -480,7 +482,11 @@ extern "C" int umic_qk_norm_mrope_kv(const umic_mrope_args* args, void* stream) 
   a.q_eps = q_eps;
   a.k_eps = k_eps;
   a.scaling = scaling;
-  // lanes of a row: a power of two, but for the 5 and 6 that head_dim 80 and 96 fill
+  // Lanes of a row: a power of two, but for the 5 and 6 that head_dim 80 and 96 fill. 16384
+  // tokens of 16 + 16 heads x 80, two axes: 37.5 us with 5 lanes, 38.7 with 8; normed, three
+  // axes, 16 + 8 + 8 heads into pages 43.5 and 46.0, written as they are 38.4 and 36.5. x 96:
+  // 38.4 with 6 lanes, 39.2 with 8; 47.0 and 46.9; 40.1 and 39.8. Other sizes keep idle lanes:
+  // no model here has them.
   const int tph = head_dim <= 64 ? 4 : head_dim == 80 ? 5 : head_dim == 96 ? 6
                   : head_dim <= 128 ? 8 : 16;
   const int at_once = 32 / tph;

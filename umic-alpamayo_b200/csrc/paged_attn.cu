@@ -20,10 +20,15 @@
 //   m, l, P        running maximum and sum of each head, fp32, base 2
 //   O^T += V^T P   V through transposing ldmatrix, P transposed in registers
 // P is fp32 split into a bf16 value and its bf16 remainder (two products, weights held to
-// 2^-17): the tensor pipe has the time. e4m3 pages are widened to fp16 in registers, which
-// holds them exactly; q is scaled by a power of two to stay inside fp16 and P by 2^15 so
-// that small weights stay normal, rounded to 2^-12. (The e4m3 form of mma.sync is made of
-// conversions and fp16 products here: more instructions, not fewer.)
+// 2^-17): the tensor pipe has the time. (Where V is infinite a remainder of 0 makes NaN.)
+// e4m3 pages are widened to fp16 in registers, which holds them exactly. q is scaled by the
+// power of two of its row's largest to stay inside fp16: what is below 2^-14 of that is held
+// to 2^-25 of it. P is held as one fp16 value times 2^15, so that small weights stay normal:
+// each is off by 2^-11 of itself at most, while their sum takes them unrounded. Two fp16
+// terms, as for bf16 pages, took 220 us for 205 (256 requests of up to 4096 tokens, 16 and 8
+// heads) and left the error against 64 bits, 0.0017 of the outputs' size by their own
+// rounding to bf16, as it was. (The e4m3 form of mma.sync is made of conversions and fp16
+// products here: more instructions, not fewer.)
 //
 // Join. A warp whose run covers a whole segment writes its rows. Otherwise it has partial
 // (m, l, O): neighbours of one CTA that share a segment join through shared memory, and
@@ -33,10 +38,14 @@
 // runs once, at the end, from a cold instruction cache.)
 //
 // Measured, both kernels, 32 query and 8 KV heads x 128: 32 requests of up to 32768 tokens
-// (2.2 GB) 346 us, 0.97 of measured HBM; 8 of 3164 tokens (104 MB) 26.6 us, of which 16 us
+// (2.2 GB) 348 us, 0.96 of measured HBM; 8 of 3164 tokens (104 MB) 26.6 us, of which 16 us
 // stream and 10 us are start, join and the spread of the warps' ends; 1 of 3164 12.9 us.
-// 256 requests of up to 4096 tokens in e4m3 pages, 16 and 8 heads (1.04 GB) 206 us: there
-// the widening (half of a tile's instructions) bounds it as much as HBM.
+// 256 requests of up to 4096 tokens in e4m3 pages, 16 and 8 heads (1.04 GB) 205 us: there
+// the widening (half of a tile's instructions) bounds it as much as HBM. 128 requests of up
+// to 4096 tokens, two query heads to a KV head, 16 KV heads of 64, 80, 96, 128 (8 of 256), in
+// bf16: 187, 243, 283, 346, 343 us, 0.81 to 0.91; in e4m3: 154, 172, 191, 217, 222 us, 0.51 to
+// 0.72. 256 of up to 4096, 4 KV heads x 128: 16 query heads to each 200 us (0.79), e4m3 167
+// (0.48); 32 to each, whose two segments read K and V twice, 348 (0.46) and 303 (0.27).
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -88,11 +97,17 @@ struct PagedArgs {
   float scale_log2;
 };
 
+// Subtiles of a tile: two for rows of up to 192 bytes, whose running maximum and shuffles
+// cost a tile the same whatever it holds (the cases of two query heads above with one: bf16
+// 200, 256, 298 us for head dims 64, 80, 96; e4m3 192, 212, 226, 254 for 64 to 128). Two of
+// rows of 256 bytes, 16 KB of K and V, would leave eight warps one stage.
 constexpr int subtiles(int d, bool e4m3) { return d * (e4m3 ? 1 : 2) <= 192 ? 2 : 1; }
 // Warps of a CTA. bf16: 8, of whose ring of three 8 KB tiles two fill while one is used
-// (head_dim 256: 4, whose accumulators fit the registers). e4m3: the work of widening,
-// twice per byte, wants 12 to hide its latencies (256 requests of up to 4096 tokens: 217 us
-// against 240 with 8), unless two column tiles' accumulators leave room for 8 only.
+// (head_dim 256: 4, whose 16 KB tiles and accumulators fit). e4m3: the work of widening,
+// twice per byte, wants 12 to hide its latencies (the cases of two query heads above, head
+// dims 64 to 256: 154, 172, 191, 217, 222 us, against 194, 196, 212, 248, 227 with 8; 16
+// query heads x 64: 185 against 216), unless two column tiles' accumulators leave room for 8
+// only.
 constexpr int warps_per_cta(int d, bool e4m3, int per) {
   return e4m3 ? (d >= 128 && per > 8 ? 8 : 12) : d == 256 ? 4 : 8;
 }
@@ -114,8 +129,6 @@ struct Shape {
   __device__ static uint32_t along(uint32_t at, int bytes) {
     return kSwizzle ? at ^ bytes : at + bytes;
   }
-  // Two subtiles a tile for rows of up to 192 bytes: the running maximum and its shuffles
-  // cost a tile the same whatever it holds.
   static constexpr int MT = subtiles(D, kE4m3);
   static constexpr int kTile = kSub * MT;                           // tokens per tile
   static constexpr int kSubBytes = 2 * kSub * kPitch;               // K, then V
@@ -1025,8 +1038,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(PagedArgs a
 }
 
 // Query heads that share a segment: 8, or 16 for wider groups, which halves the K and V
-// traffic of their segments (head_dim 256 keeps 8: accumulators of 16 would not fit the
-// registers).
+// traffic of their segments (256 requests of up to 4096 tokens, 16 query heads to each of 4 KV
+// heads x 128: 200 us against 325 with 8, e4m3 167 against 205; head_dim 256 keeps 8:
+// accumulators of 16 would not fit the registers, and 16 query heads to a KV head take 329 us,
+// 0.48 of measured HBM).
 int heads_per_segment(int group, int head_dim) { return group > 8 && head_dim <= 128 ? 16 : 8; }
 
 // CTAs of the main kernel: one per SM, fewer where the longest line that the table allows is

@@ -250,16 +250,21 @@ def qk_norm_mrope_kv(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor | 
                      k_out: torch.Tensor | None = None):
     """Per-head RMSNorm, rotary positions with several axes, and the paged K/V write.
 
-    q [T, Hq, D], k / v [T, Hk, D] bf16 (any token and head strides, D contiguous).
+    q [T, Hq, D], k / v [T, Hk, D] bf16 (D contiguous, token and head strides multiples of 8
+    elements, 16-byte aligned; so are outputs and pages, whose rows must lie apart).
     positions [axes, T] (or [T]) int32 / int64 holds one coordinate per axis -- (time,
     height, width) of an image patch, three equal ones for text -- and inv_freq [r / 2]
-    fp32 the frequencies of the r rotated elements; `sections` says how many frequencies
-    each axis turns, in runs (t..t h..h w..w) or, with interleaved, as t h w t h w ... t t.
-    cos and sin are multiplied by `scaling`. Norms run where a weight [D] is given.
+    fp32 the frequencies of the r rotated elements. `sections`, one per axis, sum to r / 2:
+    the axes turn that many frequencies each, in runs (t..t h..h w..w); with interleaved,
+    frequency i is turned by axis i % axes while i < axes * section of that axis, else by the
+    first (t h w t h w ... t t), so (24, 20, 20) turns as many of each but (10, 27, 27) turns
+    22, 21 and 21, as transformers does. cos and sin are multiplied by `scaling`. Norms run
+    where a weight [D] is given.
 
-    With k_pages / v_pages [P, Hk, page, D], k and v are written at slots [T] int32 (-1
-    skips a token; two tokens must not share a slot) and (q_out, None) is returned;
-    without, (q_out, k_out), and v is not touched. q_out may be q and k_out k.
+    With k_pages / v_pages [P, Hk, page, D], k and v are written at slots [T] int32 (one per
+    row; -1 skips a token; two tokens must not share a slot) and (q_out, None) is returned;
+    without, (q_out, k_out), and v is not touched. q_out may be q and k_out k. e4m3 pages
+    hold the fp32 value divided by its head's scale, rounded once, saturated at +-448.
     """
     if positions is None or inv_freq is None:
         raise ValueError("qk_norm_mrope_kv: positions and inv_freq are needed")
@@ -297,7 +302,11 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     [B, max_pages], kv_lens int32 [B] (read on the device). Returns out [B, Hq, D], with
     return_lse also the log of each row's sum of exponentials, fp32 [B, Hq]. Requests
     without tokens come out as zeros (lse -inf). D 64, 80, 96, 128 or 256; page a multiple
-    of 16; any number of query heads per KV head.
+    of 16; any number of query heads per KV head; strides multiples of 16 bytes. Sums are
+    fp32; weights are held to 2^-17 of themselves over bf16 pages, to 2^-11 over e4m3 ones.
+
+    There is one query row per request: a prompt that continues a cached request can be
+    planned and written, but its tokens cannot be attended here except one step each.
     """
     dev = _one_device("paged_attention", q, k_pages, v_pages, block_table, kv_lens, k_scale,
                       v_scale, out)

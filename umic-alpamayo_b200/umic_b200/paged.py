@@ -12,6 +12,12 @@ step of the same batch:
     for layer ...:
         q = cache.write(layer, q, k, v, step, positions, inv_freq, sections, ...)
         out = cache.attend(layer, q, scale)      # one new token per request
+
+A step's q, k and v have `capacity` rows: the requests' new tokens one request behind the
+other, and rows of any content behind the last. `attend` takes one query row per request,
+over all that is cached. So prompts are attended by the model's own attention, on the dense
+k and v of the step; a prompt that continues a cached request has no attention over the
+pages other than one token a step.
 """
 
 from __future__ import annotations
@@ -63,7 +69,8 @@ class PagedKVCache:
     def step(self, new_tokens: torch.Tensor, capacity: int) -> PagedPlan:
         """Advances the requests: new_tokens int32 [max_requests] on the device says how many
         tokens each appends (0: none; negative: drops that many, -kv_lens ends it).
-        `capacity` bounds the step's tokens, which are numbered request by request. Requests
+        `capacity` bounds the step's tokens, which are numbered request by request, and is
+        the number of the plan's slots and of the rows that `write` and `append` take. Requests
         that find no page, row or capacity keep their length and their tokens' slots are -1
         (umic_b200.device_errors() then holds DEVERR_PAGES). Returns the plan; its kv_lens
         is this cache's."""
@@ -89,16 +96,17 @@ class PagedKVCache:
     def write(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
               plan: PagedPlan, positions: torch.Tensor, inv_freq: torch.Tensor, sections,
               **kwargs) -> torch.Tensor:
-        """Norms and rotates q and k and writes k and v at the plan's slots; returns the
-        rotated q (qk_norm_mrope_kv's arguments)."""
+        """Norms and rotates q and k [capacity, heads, head_dim] and writes k and v at the
+        plan's slots (rows whose slot is -1 are not written); returns the rotated q
+        (qk_norm_mrope_kv's arguments; positions [axes, capacity])."""
         k_pages, v_pages = self.pages(layer)
         return qk_norm_mrope_kv(q, k, v, positions, inv_freq, sections, k_pages=k_pages,
                                 v_pages=v_pages, slots=plan.slots, **self.scales(layer),
                                 **kwargs)[0]
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, plan: PagedPlan) -> None:
-        """Writes finished keys and values [tokens, kv_heads, head_dim] at the plan's slots,
-        e.g. those of a dense prefill."""
+        """Writes finished keys and values [capacity, kv_heads, head_dim] at the plan's
+        slots, e.g. those of a dense prefill."""
         paged_kv_append(*self.pages(layer), k, v, plan.slots, **self.scales(layer))
 
     def attend(self, layer: int, q: torch.Tensor, scale: float, *,
