@@ -163,6 +163,35 @@ def test_e4m3_pages_hold_the_rounded_quotient(cuda, form):
         assert torch.equal(got[0], want)
 
 
+@pytest.mark.parametrize("rotated", [False, True])
+def test_e4m3_pages_keep_special_values(cuda, rotated):
+    """Zeros of both signs, infinities (saturated), NaN and the smallest and largest bf16
+    values, over scales from 2^-100 to 2^100 and 1e-30."""
+    big, small = torch.finfo(torch.bfloat16).max, torch.finfo(torch.bfloat16).tiny
+    x = torch.tensor([0.0, -0.0, float("inf"), -float("inf"), float("nan"), big, -big, small,
+                      -small, 448.0, -449.0, 464.0, 465.0, 1.0, -(2.0 ** -9), 2.0 ** -10])
+    scale = torch.tensor([2.0 ** -100, 1e-30, 2.0 ** -10, 1.0, 0.3, 7.0, 2.0 ** 100])
+    k = x.to(torch.bfloat16).expand(1, len(scale), 16).contiguous().to(cuda)
+    pages = torch.zeros(2, 1, len(scale), 16, 16, dtype=torch.uint8, device=cuda)
+    pool, s = pages.view(torch.float8_e4m3fn), scale.to(cuda)
+    slots = torch.tensor([2], dtype=torch.int32, device=cuda)
+    if rotated:  # pairs of a finite element and one that is not are NaN: no rotation of pairs
+        k = torch.where(k.isfinite(), k, 1.0)
+        qk_norm_mrope_kv(None, k, k, torch.zeros(1, 1, dtype=torch.int32, device=cuda),
+                         torch.ones(8, device=cuda), (8,), k_pages=pool[0], v_pages=pool[1],
+                         slots=slots, k_scale=s, v_scale=s)
+    else:
+        paged_kv_append(pool[0], pool[1], k, k, slots, k_scale=s, v_scale=s)
+    want = _stored(k[0].float().cpu(), scale[:, None])
+    got = pages[:, 0, :, 2].cpu()
+    nan = (want & 0x7f) == 0x7f
+    assert bool(((got & 0x7f)[:, nan] == 0x7f).all())
+    same = got == want
+    if rotated:  # x - y * 0 of K may lose the sign of a zero
+        same[0] |= ((got[0] | want) & 0x7f) == 0
+    assert bool((same | nan).all())
+
+
 # ------------------------------------------------------------- long walks
 
 WALKS = [

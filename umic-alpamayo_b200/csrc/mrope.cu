@@ -102,7 +102,7 @@ __device__ __forceinline__ void divide(float (&x)[8], float (&y)[8], float scale
   auto over = [scale, inv](float v) {
     // 512 saturates all the same, and the remainder of an infinity would be NaN
     const float q = fminf(fmaxf(v * inv, -512.f), 512.f);
-    return fmaf(fmaf(-q, scale, v), inv, q);
+    return fmaf(-fmaf(q, scale, -v), inv, q);  // so signed, -0 stays -0
   };
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
