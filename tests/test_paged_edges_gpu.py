@@ -345,3 +345,83 @@ def test_infinite_values_reach_their_rows(cuda, sign):
     assert not bool(out[0, 3:, 17].isfinite().any())
     out[0, 3:, 17] = clean[0, 3:, 17]
     assert torch.equal(out, clean)
+
+
+# ------------------------------------------------- optional and shared arguments
+
+def _e4m3_pool(g, pages, heads, page, d, dev):
+    x = (torch.randn(2, pages, heads, page, d, generator=g) * 3).clamp(-448, 448)
+    return x.to(torch.float8_e4m3fn).to(dev)
+
+
+@pytest.mark.parametrize("given", ["none", "k", "v"])
+def test_e4m3_pages_without_scales(cuda, given):
+    """A scale that is not given is 1, for K and V each, in the write and in the attention."""
+    g = _gen(57)
+    pool = _e4m3_pool(g, 5, 2, 16, 64, cuda)
+    other = pool.view(torch.uint8).clone().view(pool.dtype)
+    s = (0.5 + torch.rand(2, generator=g)).to(cuda)
+    one = torch.ones(2, device=cuda)
+    some = {} if given == "none" else {f"{given}_scale": s}
+    full = {"k_scale": one, "v_scale": one, **some}
+    k, v = torch.randn(2, 9, 2, 64, generator=g).to(torch.bfloat16).to(cuda)
+    slots = torch.randperm(80, generator=g)[:9].int().to(cuda)
+    paged_kv_append(pool[0], pool[1], k, v, slots, **some)
+    paged_kv_append(other[0], other[1], k, v, slots, **full)
+    assert torch.equal(pool.view(torch.uint8), other.view(torch.uint8))
+    q = torch.randn(2, 8, 64, generator=g).to(torch.bfloat16).to(cuda)
+    table = torch.tensor([[4, 1, 0], [2, 3, 0]], dtype=torch.int32, device=cuda)
+    lens = torch.tensor([40, 17], dtype=torch.int32, device=cuda)
+    a = paged_attention(q, pool[0], pool[1], table, lens, 0.1, return_lse=True, **some)
+    b = paged_attention(q, pool[0], pool[1], table, lens, 0.1, return_lse=True, **full)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_attention_tables_of_every_kind(cuda):
+    """A table of no columns, one row for all requests, rows far apart; no requests at all."""
+    g = _gen(59)
+    kp, vp = torch.randn(2, 6, 2, 16, 64, generator=g).to(torch.bfloat16).to(cuda)
+    q = torch.randn(3, 4, 64, generator=g).to(torch.bfloat16).to(cuda)
+    lens = torch.tensor([33, 48, 5], dtype=torch.int32, device=cuda)
+    row = torch.tensor([[3, 0, 5]], dtype=torch.int32, device=cuda)
+    want, lse = paged_attention(q, kp, vp, row.repeat(3, 1), lens, 0.2, return_lse=True)
+    assert torch.equal(paged_attention(q, kp, vp, row.expand(3, 3), lens, 0.2), want)
+    wide = torch.full((3, 11), -1, dtype=torch.int32, device=cuda)
+    wide[:, 4:7] = row
+    assert torch.equal(paged_attention(q, kp, vp, wide[:, 4:7], lens, 0.2), want)
+    none = torch.zeros(3, 0, dtype=torch.int32, device=cuda)
+    out, lse = paged_attention(q, kp, vp, none, torch.zeros_like(lens), 0.2, return_lse=True)
+    assert bool((out == 0).all()) and bool((lse == float("-inf")).all())
+    out, lse = paged_attention(q[:0], kp, vp, row[:0], lens[:0], 0.2, return_lse=True)
+    assert out.shape == (0, 4, 64) and lse.shape == (0, 4)
+
+
+def test_attention_over_its_own_queries(cuda):
+    """out may be q: whole, split and empty requests, the bits of a separate output."""
+    g = _gen(61)
+    for d, lens in ((64, [500, 0, 3, 16]), (80, [37, 1200, 1, 20]), (128, [90] * 40)):
+        lens = torch.tensor(lens, dtype=torch.int32)
+        b, width = len(lens), -(-int(lens.max()) // 16)
+        kp, vp = torch.randn(2, b * width, 2, 16, d, generator=g).to(torch.bfloat16).to(cuda)
+        table = torch.randperm(b * width, generator=g).int().view(b, width).to(cuda)
+        q = torch.randn(b, 8, d, generator=g).to(torch.bfloat16).to(cuda)
+        want = paged_attention(q, kp, vp, table, lens.to(cuda), 0.1)
+        got = paged_attention(q, kp, vp, table, lens.to(cuda), 0.1, out=q)
+        assert got is q and torch.equal(got, want)
+
+
+def test_first_calls_of_no_tokens(cuda):
+    """Steps and writes of no tokens leave everything as it is."""
+    from umic_b200.paged import PagedKVCache
+
+    cache = PagedKVCache.allocate(1, 4, 2, 64, 16, 3, 2, cuda)
+    cache.slab.zero_()
+    plan = cache.step(torch.zeros(3, dtype=torch.int32, device=cuda), 0)
+    x = torch.zeros(0, 2, 64, dtype=torch.bfloat16, device=cuda)
+    assert plan.slots.numel() == 0 and plan.cu_tokens.tolist() == [0] * 4
+    q = cache.write(0, x, x, x, plan, plan.positions.expand(3, -1), torch.ones(32, device=cuda),
+                    (12, 10, 10))
+    cache.append(0, x, x, plan)
+    assert q.shape == (0, 2, 64) and cache.kv_lens.tolist() == [0] * 3
+    assert cache.free_pages() == 4 and not bool(cache.slab.any())
+    assert _lib.device_errors(cuda) == 0

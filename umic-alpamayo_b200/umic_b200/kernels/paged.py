@@ -299,7 +299,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     """softmax(scale * q k^T) v of one new token per request over its pages.
 
     q [B, Hq, D] bf16 (D contiguous), pages [P, Hk, page, D], block_table int32
-    [B, max_pages], kv_lens int32 [B] (read on the device). Returns out [B, Hq, D], with
+    [B, max_pages], kv_lens int32 [B] (read on the device). Returns out [B, Hq, D] (a given
+    `out` may be q), with
     return_lse also the log of each row's sum of exponentials, fp32 [B, Hq]. Requests
     without tokens come out as zeros (lse -inf). D 64, 80, 96, 128 or 256; page a multiple
     of 16; any number of query heads per KV head; strides multiples of 16 bytes. Sums are
