@@ -283,9 +283,9 @@ UMIC_API int umic_qk_norm_mrope_kv(const umic_mrope_args* args, void* stream);
 
 /* Attention of one new token per request over its pages, grouped-query heads:
  * out[b, h] = softmax(scale * q[b, h] . k_j over j < kv_lens[b]) . v_j. q and out
- * [batch, hq, head_dim] through (sb, sh), out may be q; lse [batch, hq] fp32 (natural log of the sum
- * of exponentials; NULL = not wanted). A request without tokens comes out as zeros,
- * lse -inf. All sums are fp32. Over bf16 pages each weight is held to 2^-17 of itself;
+ * [batch, hq, head_dim] through (sb, sh), out may be q; lse [batch, hq] fp32 (natural
+ * log of the sum of exponentials; NULL = not wanted). A request without tokens comes out
+ * as zeros, lse -inf. All sums are fp32. Over bf16 pages each weight is held to 2^-17 of itself;
  * over e4m3 pages to 2^-11 (one fp16 value; the sum of weights and the lse take it in
  * fp32), and elements of q below 2^-14 of their row's largest to 2^-25 of that. A NaN of a
  * token in use reaches its rows as NaN, an infinity in V as an infinity or NaN. A table
